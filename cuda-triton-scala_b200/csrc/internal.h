@@ -60,6 +60,9 @@ enum : int {
   DEVERR_TIMEOUT_MMA = 2,
   DEVERR_TIMEOUT_EPILOGUE = 3,
   DEVERR_TIMEOUT_DRAIN = 4,
+  // An expert offset or row index read on the device lies outside its range; the kernel
+  // skipped what it names (reported as QGEMM_ERR_INVALID_ARG).
+  DEVERR_BAD_INDEX = 5,
 };
 
 // ---- the tcgen05 GEMM (w8a8_tcgen05.cu) ----
@@ -214,5 +217,44 @@ qgemm_status launch_w4a16_prefill(qgemm_stream_s* s, const void* x, const uint8_
 qgemm_status launch_w4a16_grouped(qgemm_stream_s* s, const void* x, const uint32_t* wq,
                                   const void* scales, int zp, int group, void* y, int M,
                                   int N, int K);
+
+
+// ---- linear layers with their epilogue, dense or grouped by expert ----
+// y[m, n] = act(z[m, n] + bias[n]) + residual[m, n], z = x * w^T; gated: act of the first N
+// features times the second N.  kind KIND_I8: z = (float(acc) * sw[n]) * sx[m]; KIND_BF16:
+// fp32 sums.  offsets null: one group of M rows.
+struct LinArgs {
+  int kind = KIND_I8;
+  const void* x = nullptr;         // [M, ldx]
+  const void* w = nullptr;         // [E, nw, K], nw = N or 2 N (gated: gate rows, then up rows)
+  const float* sx = nullptr;       // [M]      (KIND_I8)
+  const float* sw = nullptr;       // [E, nw]  (KIND_I8)
+  const float* bias = nullptr;     // [E, nw] or null
+  const void* residual = nullptr;  // [M, ldr] of out_dtype or null
+  void* out = nullptr;             // [M, ldc]
+  const int* offsets = nullptr;    // device int32 [E + 1]: expert e has rows offsets[e] ..
+  int E = 1;
+  int M = 0, N = 0, K = 0;
+  long long ldx = 0, ldr = 0, ldc = 0;
+  int out_dtype = QGEMM_BF16;
+  int act = QGEMM_ACT_NONE;
+  int gated = 0;
+};
+constexpr int kMaxExperts = 1024;
+bool linear_tcgen05_supported(const qgemm_device_s* d, const LinArgs& a, const char** why);
+qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a);
+qgemm_status launch_linear_simt(qgemm_stream_s* s, const LinArgs& a);
+
+// ---- routing of tokens to experts (route.cu) ----
+qgemm_status launch_route_topk(qgemm_stream_s* s, const void* logits, int in_dtype,
+                               float* weights, int* experts, int* offsets, int* rows, int T,
+                               int E, int k, int renormalize);
+// sq null: rows copied (elem bytes each); else quantised to int8 as quantize_per_token.
+qgemm_status launch_dispatch_rows(qgemm_stream_s* s, const void* x, int in_dtype,
+                                  const int* rows, void* out, float* sq, int T, int k, int K,
+                                  int R);
+qgemm_status launch_combine_rows(qgemm_stream_s* s, const void* y, int in_dtype,
+                                 const int* rows, const float* weights, const void* residual,
+                                 void* out, int out_dtype, int T, int k, int N, int R);
 
 }  // namespace qg

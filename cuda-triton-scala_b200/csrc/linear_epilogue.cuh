@@ -1,0 +1,61 @@
+// linear_epilogue.cuh -- what follows the products of a linear layer, for the SIMT and the
+// tensor-core kernels: dequantisation, bias, activation, gate, residual and the one rounding
+// to the output type.
+//     z = float(acc) * sw[n] * sx[m]   (int8: two roundings, in that order)   or the fp32 sum
+//     v = act(z + bias[n]);  gated: v = act(z_gate + b_gate) * (z_up + b_up)
+//     y = round(v + residual[m, n])
+// Everything up to the last line is fp32.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include "internal.h"
+
+namespace qg {
+namespace lin {
+
+struct Epi {
+  const float* sx;
+  const float* sw;
+  const float* bias;
+  const void* residual;
+  void* out;
+  long long ldr, ldc;
+  int N, nw;       // features, weight rows of one expert (N or 2 N)
+  int out_f32;
+  int act;
+  int vec;         // out and residual rows take 4-feature vectors (8 bytes bf16, 16 fp32)
+};
+
+// SiLU's quotient through the fast exponential: __expf is within 2 ulp + 2^-21 |x| relative,
+// far below a bf16 step and below the fp32 outputs' own summation error.
+__device__ __forceinline__ float activate(int act, float v) {
+  switch (act) {
+    case QGEMM_ACT_RELU: return v > 0.f ? v : (v != v ? v : 0.f);
+    case QGEMM_ACT_GELU: return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
+    case QGEMM_ACT_GELU_TANH:
+      return 0.5f * v * (1.f + tanhf(0.79788456080286536f * (v + 0.044715f * v * v * v)));
+    case QGEMM_ACT_SILU: return v / (1.f + __expf(-v));
+    default: return v;
+  }
+}
+
+template <int KIND>
+__device__ __forceinline__ float dequant(uint32_t word, float sw, float sx) {
+  if constexpr (KIND == KIND_I8) return __fmul_rn(__fmul_rn(__int2float_rn((int)word), sw), sx);
+  else return __uint_as_float(word);
+}
+
+__device__ __forceinline__ float load_out(const void* p, int f32, size_t i) {
+  return f32 ? static_cast<const float*>(p)[i]
+             : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+
+__device__ __forceinline__ void store_out(void* p, int f32, size_t i, float v) {
+  if (f32) static_cast<float*>(p)[i] = v;
+  else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+
+}  // namespace lin
+}  // namespace qg

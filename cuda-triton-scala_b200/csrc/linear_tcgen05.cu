@@ -1,0 +1,1011 @@
+// linear_tcgen05.cu -- linear layers with their epilogue on the sm_100a tensor cores, dense
+// or grouped by expert over ragged row counts.
+//
+//     z[m, n] = sum_k x[m, k] w[n, k]      (bf16: fp32 sums; int8: int32 sums, then scales)
+//     y[m, n] = act(z + bias[n]) + residual[m, n];  gated: act(z_gate) * z_up + residual
+//
+// Both kernels compute the transposed tile: the weights are the MMA's A operand (M = 128
+// weight rows a CTA) and the tokens its B operand.  The tokens then lie along the MMA's N,
+// which is a run-time field of the instruction descriptor: a group of 44 rows costs MMAs of
+// 48 (or 64) columns instead of a whole 128- or 256-row tile, and one token costs a 16-column
+// one.  An accumulator column is a token, a TMEM lane a feature: bias and weight scale are
+// per-lane constants, and a staging buffer [token][128 features] in shared memory turns the
+// tile so that a warp stores one token's 128 features as one contiguous run.  Gated layers
+// give each CTA 64 gate rows and the 64 up rows of the same features, so both halves of a
+// product meet in the staging buffer.
+//
+//   linear_pair_kernel    many rows: CTA pairs (tcgen05 cta_group::2), tiles of 256 weight
+//       rows x up to 256 tokens, persistent, two accumulators so that the epilogue of a tile
+//       overlaps the next tile's MMAs.  Bound by the tensor pipe.
+//   linear_stream_kernel  few rows: one CTA per tile of 128 weight rows x up to 128 tokens,
+//       persistent; a cluster of 1, 2, 4 or 8 CTAs cuts K and joins its partial sums through
+//       distributed shared memory in rank order (so no scratch, no atomics, the same bits
+//       every time).  Bound by reading the weights once.
+//
+// Experts: offsets[E + 1] are read on the device; every CTA lists the experts' tiles in
+// shared memory (prefix sums) and walks the same persistent schedule, so the host never
+// waits for the counts.
+//
+// Every barrier wait is bounded; one that runs out records a code in the device error word
+// and the CTA drains its copies and MMAs, frees TMEM and returns.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <cstring>
+#include <mutex>
+
+#include "linear_epilogue.cuh"
+#include "ptx.cuh"
+
+namespace qg {
+namespace lin {
+
+constexpr int BK = 128;         // bytes of K a stage: one 128-byte swizzle row
+constexpr int UMMA_K = 32;      // bytes of K an MMA
+constexpr int WROWS = 128;      // weight rows of a CTA's tile
+constexpr int W_BYTES = WROWS * BK;          // 16 KB
+constexpr int CHUNK = 16;                    // tokens of a staging buffer
+constexpr int CHUNK_BYTES = CHUNK * WROWS * 4;
+constexpr int SMEM_MAX = 232448;             // 227 KB
+constexpr int BAR_BYTES = 512;
+constexpr int MAX_STAGES = 12;
+
+struct Params {
+  Epi ep;
+  const int* offsets;
+  int E, M;
+  int num_k_blocks;
+  int tok_max;      // tokens of a tile at most
+  int tok_round;    // tokens of a tile are a multiple of this (MMA N)
+  int num_w_blocks; // weight blocks of an expert
+  int feats;        // features of a weight block of one CTA: 128, gated 64
+  int stages;
+  int csize;        // CTAs of a cluster (stream kernel)
+  int* err;
+  unsigned long long wait_ns;
+};
+
+// The experts' rows and tiles, in shared memory.
+struct Table {
+  int* row0;  // [E] first row
+  int* cnt;   // [E] rows (0 where the offsets are not usable)
+  int* pref;  // [E + 1] tiles before the expert
+};
+
+struct Tile {
+  int e, wb;   // expert, weight block
+  int t0, n;   // first row of x / out, rows
+};
+
+__device__ __forceinline__ int blocks_of(const Params& p, int cnt) {
+  return (cnt + p.tok_max - 1) / p.tok_max;
+}
+
+// All threads: fills the table.  Offsets that are not 0 <= o[e] <= o[e+1] <= M name no rows.
+__device__ __forceinline__ void fill_table(const Params& p, const Table& tb) {
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
+    int o0 = 0, o1 = p.M;
+    if (p.offsets) {
+      o0 = p.offsets[e];
+      o1 = p.offsets[e + 1];
+      if (o0 < 0 || o1 < o0 || o1 > p.M) {
+        if (p.err && blockIdx.x == 0) atomicCAS(p.err, 0, DEVERR_BAD_INDEX);
+        o0 = o1 = 0;
+      }
+    }
+    tb.row0[e] = o0;
+    tb.cnt[e] = o1 - o0;
+    tb.pref[e] = blocks_of(p, o1 - o0) * p.num_w_blocks;
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {  // exclusive scan, a run of experts a lane
+    const int lane = threadIdx.x;
+    const int chunk = (p.E + 31) / 32, e0 = min(p.E, lane * chunk), e1 = min(p.E, e0 + chunk);
+    int sum = 0;
+    for (int e = e0; e < e1; ++e) sum += tb.pref[e];
+    int run = sum;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, run, off);
+      if (lane >= off) run += o;
+    }
+    if (lane == 31) tb.pref[p.E] = run;
+    run -= sum;
+    for (int e = e0; e < e1; ++e) {
+      const int c = tb.pref[e];
+      tb.pref[e] = run;
+      run += c;
+    }
+  }
+  __syncthreads();
+}
+
+// Tile `t` of the schedule.  An expert's rows are cut into blocks of equal size (rounded up
+// to tok_round).  Order inside an expert: bands of `band` token blocks; in a band the token
+// block runs fastest, so CTAs that work at the same time share weights and tokens in L2.
+__device__ __forceinline__ Tile tile_of(const Params& p, const Table& tb, int t, int band) {
+  int e = 0;
+  if (p.E > 1) {  // the last expert whose first tile is <= t (experts without rows have none)
+    int lo = 0, hi = p.E;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (tb.pref[mid] <= t) lo = mid; else hi = mid;
+    }
+    e = lo;
+  }
+  const int idx = t - tb.pref[e], cnt = tb.cnt[e];
+  const int nblk = blocks_of(p, cnt);
+  const int blk = (((cnt + nblk - 1) / nblk) + p.tok_round - 1) / p.tok_round * p.tok_round;
+  const int per_band = band * p.num_w_blocks;
+  const int b = idx / per_band, in = idx - b * per_band;
+  const int rows = min(nblk - b * band, band);
+  Tile r;
+  r.e = e;
+  r.wb = in / rows;
+  const int first = (b * band + in % rows) * blk;
+  r.t0 = tb.row0[e] + first;
+  r.n = max(0, min(blk, cnt - first));
+  return r;
+}
+
+__device__ __forceinline__ void report(int* err, int code, volatile int* abort_flag) {
+  *abort_flag = 1;
+  if (err) atomicCAS(err, 0, code);
+}
+
+// As report(), and raises the abort flags of the other CTAs of the cluster, so that their
+// waits give up at once.
+__device__ __forceinline__ void report_cluster(int* err, int code, volatile int* abort_flag,
+                                               int csize) {
+  report(err, code, abort_flag);
+  const uint32_t here = ptx::smem_u32(const_cast<int*>(abort_flag));
+  for (int c = 0; c < csize; ++c) ptx::st_cluster_u32(ptx::map_to_rank(here, c), 1u);
+}
+
+// ---- finishing four features of a token ---------------------------------------------------
+
+// Per-lane constants of a tile: this lane's four features (and, gated, their up rows).
+template <bool GATED>
+struct Feat {
+  int n;            // first feature, N or more: none
+  float sg[4], bg[4], su[GATED ? 4 : 1], bu[GATED ? 4 : 1];
+};
+
+template <int KIND, bool GATED>
+__device__ __forceinline__ void load_feat(const Epi& ep, int e, int n, Feat<GATED>& f) {
+  f.n = n;
+  const size_t base = (size_t)e * ep.nw + n;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool in = n + i < ep.N;
+    f.sg[i] = KIND == KIND_I8 && in ? __ldg(ep.sw + base + i) : 0.f;
+    f.bg[i] = ep.bias && in ? __ldg(ep.bias + base + i) : 0.f;
+    if constexpr (GATED) {
+      f.su[i] = KIND == KIND_I8 && in ? __ldg(ep.sw + base + ep.N + i) : 0.f;
+      f.bu[i] = ep.bias && in ? __ldg(ep.bias + base + ep.N + i) : 0.f;
+    }
+  }
+}
+
+// The residual of four features of a row, fetched before the products are needed.
+__device__ __forceinline__ void load_residual(const Epi& ep, int row, int n, float (&r)[4]) {
+  if (!ep.residual) return;
+  const size_t at = (size_t)row * ep.ldr + n;
+  if (ep.vec && n + 4 <= ep.N) {
+    if (ep.out_f32) {
+      const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(ep.residual) + at);
+      r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w;
+    } else {
+      const uint2 u = *reinterpret_cast<const uint2*>(
+          static_cast<const __nv_bfloat16*>(ep.residual) + at);
+      r[0] = __uint_as_float(u.x << 16);
+      r[1] = __uint_as_float(u.x & 0xffff0000u);
+      r[2] = __uint_as_float(u.y << 16);
+      r[3] = __uint_as_float(u.y & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      r[i] = n + i < ep.N ? load_out(ep.residual, ep.out_f32, at + i) : 0.f;
+  }
+}
+
+// ACT is a compile-time choice: the switch sits outside the loops.
+template <int KIND, bool GATED, int ACT>
+__device__ __forceinline__ void finish4(const Epi& ep, const Feat<GATED>& f, int row, float sx,
+                                        const uint32_t (&g)[4], const uint32_t (&u)[4],
+                                        const float (&res)[4]) {
+  float v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[i] = activate(ACT, __fadd_rn(dequant<KIND>(g[i], f.sg[i], sx), f.bg[i]));
+    if constexpr (GATED)
+      v[i] = __fmul_rn(v[i], __fadd_rn(dequant<KIND>(u[i], f.su[i], sx), f.bu[i]));
+  }
+  if (ep.residual) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __fadd_rn(v[i], res[i]);
+  }
+  const size_t at = (size_t)row * ep.ldc + f.n;
+  if (ep.vec && f.n + 4 <= ep.N) {
+    if (ep.out_f32) {
+      *reinterpret_cast<float4*>(static_cast<float*>(ep.out) + at) =
+          make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+      const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]);
+      const __nv_bfloat162 b = __floats2bfloat162_rn(v[2], v[3]);
+      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(ep.out) + at) =
+          make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (f.n + i < ep.N) store_out(ep.out, ep.out_f32, at + i, v[i]);
+  }
+}
+
+// Calls fn with the activation as a compile-time constant.
+template <typename F>
+__device__ __forceinline__ void with_act(int act, F&& fn) {
+  switch (act) {
+    case QGEMM_ACT_RELU: fn(std::integral_constant<int, QGEMM_ACT_RELU>()); break;
+    case QGEMM_ACT_GELU: fn(std::integral_constant<int, QGEMM_ACT_GELU>()); break;
+    case QGEMM_ACT_GELU_TANH: fn(std::integral_constant<int, QGEMM_ACT_GELU_TANH>()); break;
+    case QGEMM_ACT_SILU: fn(std::integral_constant<int, QGEMM_ACT_SILU>()); break;
+    default: fn(std::integral_constant<int, QGEMM_ACT_NONE>()); break;
+  }
+}
+
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+__device__ __forceinline__ void st_shared_u32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
+// ---- the CTA-pair kernel -------------------------------------------------------------------
+namespace pair {
+constexpr int TOK = 256;                  // tokens of a tile at most (MMA N)
+constexpr int TOK_BYTES = (TOK / 2) * BK; // each CTA holds half the tokens: 16 KB a stage
+constexpr int STAGE_BYTES = W_BYTES + TOK_BYTES;
+constexpr int BOX = 64;                   // token rows of a TMA box
+constexpr int EPI_WARPS = 8;              // two groups of four (one warp a TMEM lane quadrant)
+constexpr int THREADS = 64 + 32 * EPI_WARPS;
+constexpr int STG_BYTES = 2 * 2 * CHUNK_BYTES;  // two buffers for each group
+constexpr int BAND = 8;
+}  // namespace pair
+
+// Item i of pair `pid`: a whole tile in the full rounds; in the last round the `rest` tiles
+// that are left are cut along their tokens into up to four parts, one a pair, so that the
+// round takes a part's time.  Returns false when there is none; an item may have no tokens.
+__device__ __forceinline__ bool pair_item(const Params& p, const Table& tb, int pid, int npairs,
+                                          int i, Tile& r) {
+  const int T = tb.pref[p.E];
+  const int rounds = T / npairs, rest = T - rounds * npairs;
+  if (i < rounds) {
+    r = tile_of(p, tb, pid + i * npairs, pair::BAND);
+    return true;
+  }
+  if (i > rounds || rest == 0) return false;
+  const int parts = min(4, npairs / rest);
+  if (pid >= rest * parts) return false;
+  r = tile_of(p, tb, rounds * npairs + pid / parts, pair::BAND);
+  if (parts > 1) {
+    const int w = ((r.n + parts - 1) / parts + p.tok_round - 1) / p.tok_round * p.tok_round;
+    const int first = (pid % parts) * w;
+    r.n = max(0, min(w, r.n - first));
+    r.t0 += first;
+  }
+  return true;
+}
+
+template <int KIND, bool GATED>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
+    linear_pair_kernel(const __grid_constant__ CUtensorMap tmW,
+                       const __grid_constant__ CUtensorMap tmX, const Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_base = ptx::smem_u32(smem_raw);
+  const uint32_t base = (raw_base + 1023u) & ~1023u;
+  uint8_t* gbase = smem_raw + (base - raw_base);
+  const int S = p.stages;
+  const uint32_t stg_base = base + S * pair::STAGE_BYTES;
+  const uint32_t bar_base = stg_base + pair::STG_BYTES;
+  uint8_t* gbar = gbase + S * pair::STAGE_BYTES + pair::STG_BYTES;
+  auto full_bar = [&](int s) { return bar_base + 8u * s; };
+  auto empty_bar = [&](int s) { return bar_base + 8u * (MAX_STAGES + s); };
+  auto tfull_bar = [&](int a) { return bar_base + 8u * (2 * MAX_STAGES + a); };
+  auto tempty_bar = [&](int a) { return bar_base + 8u * (2 * MAX_STAGES + 2 + a); };
+  const uint32_t drain_bar = bar_base + 8u * (2 * MAX_STAGES + 4);
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gbar + 8 * (2 * MAX_STAGES + 5));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(gbar + 8 * (2 * MAX_STAGES + 5) + 4);
+  Table tb;
+  tb.row0 = reinterpret_cast<int*>(gbar + BAR_BYTES);
+  tb.cnt = tb.row0 + p.E;
+  tb.pref = tb.cnt + p.E;
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t rank = ptx::cluster_ctarank();
+  const int pid = blockIdx.x / 2, npairs = gridDim.x / 2;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      ptx::mbar_init(full_bar(s), 1);
+      ptx::mbar_init(empty_bar(s), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      ptx::mbar_init(tfull_bar(a), 1);
+      ptx::mbar_init(tempty_bar(a), 2 * pair::EPI_WARPS);
+    }
+    ptx::mbar_init(drain_bar, 1);
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+    ptx::grid_launch_dependents();
+    ptx::prefetch_tmap(&tmW);
+    ptx::prefetch_tmap(&tmX);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc_pair(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
+    ptx::tmem_relinquish_pair();
+  }
+  ptx::grid_dependency_wait();  // the offsets, and everything below, may be the previous kernel's
+  fill_table(p, tb);
+  ptx::tc_fence_before();
+  ptx::cluster_sync_all();
+  ptx::tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  Tile it_;
+
+  if (warp == 0) {
+    // ---------------- TMA producer (both CTAs) ----------------
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      long long issued = 0;
+      bool ok = true;
+      for (int item = 0; ok && pair_item(p, tb, pid, npairs, item, it_); ++item) {
+        if (it_.n == 0) continue;
+        const int half = (it_.n + p.tok_round - 1) / p.tok_round * p.tok_round / 2;
+        const int boxes = (half + pair::BOX - 1) / pair::BOX;
+        const uint32_t tx = 2u * (W_BYTES + (uint32_t)boxes * pair::BOX * BK);
+        const int x0 = it_.t0 + (int)rank * half;
+        // this CTA's weight rows: 128 of the block's 256, or 64 gate and 64 up rows
+        const int w0 = it_.e * p.ep.nw + (it_.wb * 2 + (int)rank) * p.feats;
+        for (int kb = 0; kb < p.num_k_blocks; ++kb) {
+          if (!ptx::mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.wait_ns)) {
+            if (!*abort_flag) report_cluster(p.err, DEVERR_TIMEOUT_PRODUCER, abort_flag, 2);
+            ok = false;
+            break;
+          }
+          const uint32_t sw = base + stage * pair::STAGE_BYTES, sx = sw + W_BYTES;
+          const uint32_t fb = ptx::map_to_rank(full_bar(stage), 0);
+          if (rank == 0) ptx::mbar_arrive_expect_tx(full_bar(stage), tx);
+          ptx::tma_load_2d_pair(sw, &tmW, fb, kb * BK, w0);
+          if (GATED) ptx::tma_load_2d_pair(sw + W_BYTES / 2, &tmW, fb, kb * BK, w0 + p.ep.N);
+          for (int b = 0; b < boxes; ++b)
+            ptx::tma_load_2d_pair(sx + b * pair::BOX * BK, &tmX, fb, kb * BK, x0 + b * pair::BOX);
+          ++issued;
+          if (++stage == S) { stage = 0; phase ^= 1u; }
+        }
+      }
+      // Drain: the even CTA's full barriers count both CTAs' copies.
+      if (rank == 0) {
+        for (long long f = (issued > S ? issued - S : 0); f < issued; ++f) {
+          if (!ptx::mbar_wait(full_bar((int)(f % S)), (uint32_t)((f / S) & 1), nullptr, p.wait_ns)) {
+            report_cluster(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag, 2);
+            break;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer (even CTA) ----------------
+    if (lane == 0 && rank == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int it = 0;
+      bool ok = true, issued_any = false;
+      for (int item = 0; ok && pair_item(p, tb, pid, npairs, item, it_); ++item) {
+        if (it_.n == 0) continue;
+        const int ncol = (it_.n + p.tok_round - 1) / p.tok_round * p.tok_round;
+        const uint32_t idesc = KIND == KIND_BF16 ? ptx::idesc_bf16(256, ncol)
+                                                 : ptx::idesc_i8(256, ncol, false, false);
+        const int a = it & 1;
+        if (!ptx::mbar_wait(tempty_bar(a), (uint32_t)((it >> 1) & 1) ^ 1u, abort_flag, p.wait_ns)) {
+          if (!*abort_flag) report_cluster(p.err, DEVERR_TIMEOUT_MMA, abort_flag, 2);
+          ok = false;
+          break;
+        }
+        ++it;
+        ptx::tc_fence_after();
+        const uint32_t d_tmem = tmem_base + (uint32_t)(a * 256);
+        for (int kb = 0; kb < p.num_k_blocks; ++kb) {
+          if (!ptx::mbar_wait(full_bar(stage), phase, abort_flag, p.wait_ns)) {
+            if (!*abort_flag) report_cluster(p.err, DEVERR_TIMEOUT_MMA, abort_flag, 2);
+            ok = false;
+            break;
+          }
+          ptx::tc_fence_after();
+          const uint32_t sw = base + stage * pair::STAGE_BYTES, sx = sw + W_BYTES;
+#pragma unroll
+          for (int kk = 0; kk < BK / UMMA_K; ++kk) {
+            const uint64_t adesc = ptx::smem_desc_sw128(sw + kk * UMMA_K, 16, 1024);
+            const uint64_t bdesc = ptx::smem_desc_sw128(sx + kk * UMMA_K, 16, 1024);
+            const uint32_t accum = (kb | kk) != 0 ? 1u : 0u;
+            if constexpr (KIND == KIND_BF16) ptx::umma_bf16_pair(d_tmem, adesc, bdesc, idesc, accum);
+            else ptx::umma_i8_pair(d_tmem, adesc, bdesc, idesc, accum);
+          }
+          ptx::umma_commit_pair(empty_bar(stage), 0x3);
+          issued_any = true;
+          if (++stage == S) { stage = 0; phase ^= 1u; }
+        }
+        if (ok) ptx::umma_commit_pair(tfull_bar(a), 0x3);
+      }
+      if (!ok && issued_any) {
+        ptx::umma_commit_pair(drain_bar, 0x1);
+        if (!ptx::mbar_wait(drain_bar, 0, nullptr, p.wait_ns))
+          report_cluster(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag, 2);
+      }
+    }
+  } else {
+    // ---------------- epilogue (both CTAs, two groups of four warps) ----------------
+    const int q = warp & 3;             // TMEM lane quadrant: features 32 q ..
+    const int grp = (warp - 2) / 4;     // chunks c with c % 2 == grp
+    const int w4 = (warp - 2) % 4;      // warp of the group
+    const uint32_t stg = stg_base + (uint32_t)grp * 2 * CHUNK_BYTES;
+    const uint32_t te0 = ptx::map_to_rank(tempty_bar(0), 0);
+    const uint32_t te1 = ptx::map_to_rank(tempty_bar(1), 0);
+    const Epi& ep = p.ep;
+    int it = 0, seq = 0;
+    for (int item = 0; pair_item(p, tb, pid, npairs, item, it_); ++item) {
+      if (it_.n == 0) continue;
+      const int a = it & 1;
+      const int nf = (it_.wb * 2 + (int)rank) * p.feats + 4 * (GATED ? lane % 16 : lane);
+      Feat<GATED> f;
+      load_feat<KIND, GATED>(ep, it_.e, nf, f);
+      // a warp whose wait ran out keeps the group's barrier sequence and stores nothing
+      bool ok = ptx::mbar_wait_sleep(tfull_bar(a), (uint32_t)((it >> 1) & 1), abort_flag, p.wait_ns);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok && lane == 0 && !*abort_flag)
+        report_cluster(p.err, DEVERR_TIMEOUT_EPILOGUE, abort_flag, 2);
+      ++it;
+      ptx::tc_fence_after();
+      const int chunks = (it_.n + CHUNK - 1) / CHUNK;
+      with_act(ep.act, [&](auto act) {
+        for (int c = grp; c < chunks; c += 2, ++seq) {
+          const uint32_t buf = stg + (uint32_t)(seq & 1) * CHUNK_BYTES;
+          uint32_t r[16];
+          if (ok) {
+            ptx::tmem_ld_32x32b_x16(
+                tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * 256 + c * CHUNK), r);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) r[j] = 0u;
+          }
+          // the rows this lane finishes: scales and residuals, while the load is under way
+          constexpr int ROWS = GATED ? 2 : 4;
+          float sx[ROWS], res[ROWS][4];
+          int row[ROWS];
+#pragma unroll
+          for (int i = 0; i < ROWS; ++i) {
+            const int t = GATED ? w4 * 2 + lane / 16 + 8 * i : w4 + 4 * i;
+            const bool in = ok && c * CHUNK + t < it_.n && f.n < ep.N;
+            row[i] = in ? it_.t0 + c * CHUNK + t : -1;
+            sx[i] = 1.f;
+            if (in) {
+              if (KIND == KIND_I8) sx[i] = __ldg(ep.sx + row[i]);
+              load_residual(ep, row[i], f.n, res[i]);
+            }
+          }
+          ptx::tmem_wait_ld();
+          if (c + 2 >= chunks) {  // this warp has read its last columns of the accumulator
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive_remote(a ? te1 : te0);
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            st_shared_u32(buf + (uint32_t)(j * WROWS + q * 32 + lane) * 4u, r[j]);
+          // one barrier a chunk: the buffer written next is the other one, which every warp
+          // of the group has finished reading before it arrives here
+          ptx::named_bar_sync(1 + grp, 128);
+#pragma unroll
+          for (int i = 0; i < ROWS; ++i) {
+            const int t = GATED ? w4 * 2 + lane / 16 + 8 * i : w4 + 4 * i;
+            const uint32_t at = buf + (uint32_t)(t * WROWS + 4 * (GATED ? lane % 16 : lane)) * 4u;
+            const uint4 gv = ld_shared_v4(at);
+            const uint32_t g[4] = {gv.x, gv.y, gv.z, gv.w};
+            uint32_t u[4] = {0u, 0u, 0u, 0u};
+            if (GATED) {
+              const uint4 uv = ld_shared_v4(at + 64 * 4);
+              u[0] = uv.x; u[1] = uv.y; u[2] = uv.z; u[3] = uv.w;
+            }
+            if (row[i] >= 0)
+              finish4<KIND, GATED, decltype(act)::value>(ep, f, row[i], sx[i], g, u, res[i]);
+          }
+        }
+      });
+      if (grp >= chunks) {  // no chunk of this tile is this group's
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive_remote(a ? te1 : te0);
+      }
+    }
+  }
+
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::cluster_sync_all();
+  ptx::tc_fence_after();
+  if (warp == 1) {
+    __syncwarp();
+    ptx::tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
+// ---- the streaming kernel ------------------------------------------------------------------
+namespace strm {  // tiles of 16, 32, 64 or 128 tokens at most (Params::tok_max)
+constexpr int THREADS = 192;   // producer, MMA issuer, four epilogue warps
+constexpr int BAND = 1 << 20;  // token blocks run fastest: neighbours share the weights
+}  // namespace strm
+
+template <int KIND, bool GATED>
+__global__ void __launch_bounds__(strm::THREADS, 1)
+    linear_stream_kernel(const __grid_constant__ CUtensorMap tmW,
+                         const __grid_constant__ CUtensorMap tmX, const Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_base = ptx::smem_u32(smem_raw);
+  const uint32_t base = (raw_base + 1023u) & ~1023u;
+  uint8_t* gbase = smem_raw + (base - raw_base);
+  const int S = p.stages, TOK = p.tok_max, C = p.csize;
+  const int box = TOK < 32 ? TOK : 32;  // token rows of a TMA box
+  const uint32_t stage_bytes = (uint32_t)(W_BYTES + TOK * BK);
+  // partial sums of this rank's tokens: [source rank][TOK / C tokens][128 features] words
+  const uint32_t recv = base + S * stage_bytes;
+  const uint32_t bar_base = recv + (uint32_t)TOK * WROWS * 4u;
+  uint8_t* gbar = gbase + (bar_base - base);
+  auto full_bar = [&](int s) { return bar_base + 8u * s; };
+  auto empty_bar = [&](int s) { return bar_base + 8u * (MAX_STAGES + s); };
+  auto tfull_bar = [&](int a) { return bar_base + 8u * (2 * MAX_STAGES + a); };
+  auto tempty_bar = [&](int a) { return bar_base + 8u * (2 * MAX_STAGES + 2 + a); };
+  const uint32_t drain_bar = bar_base + 8u * (2 * MAX_STAGES + 4);
+  const uint32_t rfull_bar = bar_base + 8u * (2 * MAX_STAGES + 5);   // partial sums are in
+  const uint32_t rempty_bar = bar_base + 8u * (2 * MAX_STAGES + 6);  // every rank has read its
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gbar + 8 * (2 * MAX_STAGES + 7));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(gbar + 8 * (2 * MAX_STAGES + 7) + 4);
+  Table tb;
+  tb.row0 = reinterpret_cast<int*>(gbar + BAR_BYTES);
+  tb.cnt = tb.row0 + p.E;
+  tb.pref = tb.cnt + p.E;
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int rank = C > 1 ? (int)ptx::cluster_ctarank() : 0;
+  const int cid = blockIdx.x / C, nclusters = gridDim.x / C;
+  const uint32_t tmem_cols = TOK < 16 ? 32u : 2u * TOK;  // TOK is 16, 32, 64 or 128
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      ptx::mbar_init(full_bar(s), 1);
+      ptx::mbar_init(empty_bar(s), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      ptx::mbar_init(tfull_bar(a), 1);
+      ptx::mbar_init(tempty_bar(a), 4);
+    }
+    ptx::mbar_init(drain_bar, 1);
+    ptx::mbar_init(rfull_bar, 4 * C);
+    ptx::mbar_init(rempty_bar, 4 * C);
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+    ptx::grid_launch_dependents();
+    ptx::prefetch_tmap(&tmW);
+    ptx::prefetch_tmap(&tmX);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), tmem_cols);
+    ptx::tmem_relinquish();
+  }
+  ptx::grid_dependency_wait();
+  fill_table(p, tb);
+  ptx::tc_fence_before();
+  if (C > 1) ptx::cluster_sync_all(); else __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int T = tb.pref[p.E];
+  const int kb0 = (int)((long long)p.num_k_blocks * rank / C);
+  const int kb1 = (int)((long long)p.num_k_blocks * (rank + 1) / C);
+
+  if (warp == 0) {
+    // ---------------- TMA producer ----------------
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      long long issued = 0;
+      bool ok = true;
+      for (int tile = cid; ok && tile < T; tile += nclusters) {
+        const Tile t = tile_of(p, tb, tile, strm::BAND);
+        if (t.n == 0) continue;
+        const int boxes = (t.n + box - 1) / box;
+        const uint32_t tx = W_BYTES + (uint32_t)(boxes * box * BK);
+        const int w0 = t.e * p.ep.nw + t.wb * p.feats;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!ptx::mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.wait_ns)) {
+            if (!*abort_flag) report_cluster(p.err, DEVERR_TIMEOUT_PRODUCER, abort_flag, C);
+            ok = false;
+            break;
+          }
+          const uint32_t sw = base + stage * stage_bytes, sx = sw + W_BYTES;
+          ptx::mbar_arrive_expect_tx(full_bar(stage), tx);
+          ptx::tma_load_2d(sw, &tmW, full_bar(stage), kb * BK, w0);
+          if (GATED) ptx::tma_load_2d(sw + W_BYTES / 2, &tmW, full_bar(stage), kb * BK, w0 + p.ep.N);
+          for (int b = 0; b < boxes; ++b)
+            ptx::tma_load_2d(sx + b * box * BK, &tmX, full_bar(stage), kb * BK, t.t0 + b * box);
+          ++issued;
+          if (++stage == S) { stage = 0; phase ^= 1u; }
+        }
+      }
+      for (long long f = (issued > S ? issued - S : 0); f < issued; ++f) {
+        if (!ptx::mbar_wait(full_bar((int)(f % S)), (uint32_t)((f / S) & 1), nullptr, p.wait_ns)) {
+          report_cluster(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag, C);
+          break;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer ----------------
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int it = 0;
+      bool ok = true, issued_any = false;
+      for (int tile = cid; ok && tile < T; tile += nclusters) {
+        const Tile t = tile_of(p, tb, tile, strm::BAND);
+        if (t.n == 0) continue;
+        const int ncol = (t.n + 15) / 16 * 16;
+        const uint32_t idesc = KIND == KIND_BF16 ? ptx::idesc_bf16(128, ncol)
+                                                 : ptx::idesc_i8(128, ncol, false, false);
+        const int a = it & 1;
+        if (!ptx::mbar_wait(tempty_bar(a), (uint32_t)((it >> 1) & 1) ^ 1u, abort_flag, p.wait_ns)) {
+          if (!*abort_flag) report_cluster(p.err, DEVERR_TIMEOUT_MMA, abort_flag, C);
+          ok = false;
+          break;
+        }
+        ++it;
+        ptx::tc_fence_after();
+        const uint32_t d_tmem = tmem_base + (uint32_t)(a * TOK);
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!ptx::mbar_wait(full_bar(stage), phase, abort_flag, p.wait_ns)) {
+            if (!*abort_flag) report_cluster(p.err, DEVERR_TIMEOUT_MMA, abort_flag, C);
+            ok = false;
+            break;
+          }
+          ptx::tc_fence_after();
+          const uint32_t sw = base + stage * stage_bytes, sx = sw + W_BYTES;
+#pragma unroll
+          for (int kk = 0; kk < BK / UMMA_K; ++kk) {
+            const uint64_t adesc = ptx::smem_desc_sw128(sw + kk * UMMA_K, 16, 1024);
+            const uint64_t bdesc = ptx::smem_desc_sw128(sx + kk * UMMA_K, 16, 1024);
+            const uint32_t accum = (kb != kb0 || kk != 0) ? 1u : 0u;
+            if constexpr (KIND == KIND_BF16) ptx::umma_bf16(d_tmem, adesc, bdesc, idesc, accum);
+            else ptx::umma_i8(d_tmem, adesc, bdesc, idesc, accum);
+          }
+          ptx::umma_commit(empty_bar(stage));
+          issued_any = true;
+          if (++stage == S) { stage = 0; phase ^= 1u; }
+        }
+        if (ok) ptx::umma_commit(tfull_bar(a));
+      }
+      if (!ok && issued_any) {
+        ptx::umma_commit(drain_bar);
+        if (!ptx::mbar_wait(drain_bar, 0, nullptr, p.wait_ns))
+          report_cluster(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag, C);
+      }
+    }
+  } else {
+    // ---------------- epilogue ----------------
+    const int q = warp & 3;
+    const Epi& ep = p.ep;
+    const int slot = TOK / C;  // tokens of a rank's slice at most
+    int it = 0;
+    bool ok = true;
+    for (int tile = cid; ok && tile < T; tile += nclusters) {
+      const Tile t = tile_of(p, tb, tile, strm::BAND);
+      if (t.n == 0) continue;
+      const int a = it & 1;
+      const uint32_t xphase = (uint32_t)(it & 1);  // of the exchange barriers, one use a tile
+      const int per = (t.n + C - 1) / C;           // rank r finishes tokens r * per ..
+      const int nf = t.wb * p.feats + 4 * (GATED ? lane % 16 : lane);
+      Feat<GATED> f;
+      load_feat<KIND, GATED>(ep, t.e, nf, f);
+      ok = ptx::mbar_wait(tfull_bar(a), (uint32_t)((it >> 1) & 1), abort_flag, p.wait_ns);
+      ++it;
+      // every rank has read the partial sums of the tile before
+      ok = ok && ptx::mbar_wait_acquire_cluster(rempty_bar, xphase ^ 1u, abort_flag, p.wait_ns);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) {
+        if (lane == 0 && !*abort_flag) report_cluster(p.err, DEVERR_TIMEOUT_EPILOGUE, abort_flag, C);
+        break;
+      }
+      ptx::tc_fence_after();
+      // push each token's 32 sums of this warp to the rank that finishes the token
+      int dst = 0, tl = 0;
+      uint32_t to = ptx::map_to_rank(recv, 0) + (uint32_t)((rank * slot) * WROWS + q * 32 + lane) * 4u;
+      for (int c = 0; c < t.n; c += 16) {
+        uint32_t r[16];
+        ptx::tmem_ld_32x32b_x16(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * TOK + c), r);
+        ptx::tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          if (c + j < t.n) {
+            ptx::st_cluster_u32(to, r[j]);
+            to += WROWS * 4u;
+            if (++tl == per) {
+              tl = 0;
+              ++dst;
+              if (dst < C)
+                to = ptx::map_to_rank(recv, dst) +
+                     (uint32_t)((rank * slot) * WROWS + q * 32 + lane) * 4u;
+            }
+          }
+        }
+      }
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(tempty_bar(a));
+      if (lane < C) ptx::mbar_arrive_release_cluster(ptx::map_to_rank(rfull_bar, lane));
+      ok = ptx::mbar_wait_acquire_cluster(rfull_bar, xphase, abort_flag, p.wait_ns);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) {
+        if (lane == 0 && !*abort_flag) report_cluster(p.err, DEVERR_TIMEOUT_EPILOGUE, abort_flag, C);
+        break;
+      }
+      const int mine = max(0, min(per, t.n - rank * per));
+      with_act(ep.act, [&](auto act) {
+        const int step = GATED ? 8 : 4;
+        for (int l = GATED ? (warp - 2) * 2 + lane / 16 : warp - 2; l < mine; l += step) {
+          const int row = t.t0 + rank * per + l;
+          if (f.n >= ep.N) continue;
+          float sx = 1.f, res[4];
+          if (KIND == KIND_I8) sx = __ldg(ep.sx + row);
+          load_residual(ep, row, f.n, res);
+          uint32_t g[4] = {0u, 0u, 0u, 0u}, u[4] = {0u, 0u, 0u, 0u};
+          for (int c = 0; c < C; ++c) {
+            const uint32_t at =
+                recv + (uint32_t)((c * slot + l) * WROWS + 4 * (GATED ? lane % 16 : lane)) * 4u;
+            const uint4 v = ld_shared_v4(at);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              g[i] = KIND == KIND_I8 ? g[i] + w[i]
+                                     : __float_as_uint(__fadd_rn(__uint_as_float(g[i]), __uint_as_float(w[i])));
+            if (GATED) {
+              const uint4 v2 = ld_shared_v4(at + 64 * 4);
+              const uint32_t w2[4] = {v2.x, v2.y, v2.z, v2.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                u[i] = KIND == KIND_I8 ? u[i] + w2[i]
+                                       : __float_as_uint(__fadd_rn(__uint_as_float(u[i]), __uint_as_float(w2[i])));
+            }
+          }
+          finish4<KIND, GATED, decltype(act)::value>(ep, f, row, sx, g, u, res);
+        }
+      });
+      __syncwarp();
+      if (lane < C) ptx::mbar_arrive_release_cluster(ptx::map_to_rank(rempty_bar, lane));
+    }
+  }
+
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (C > 1) ptx::cluster_sync_all();  // no CTA leaves while another writes or arrives in it
+  ptx::tc_fence_after();
+  if (warp == 1) {
+    __syncwarp();
+    ptx::tmem_dealloc(tmem_base, tmem_cols);
+  }
+}
+
+// ---- host side -----------------------------------------------------------------------------
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(p);
+  });
+  return fn;
+}
+
+// Byte map of `rows` rows of `width` bytes, `pitch` apart; boxes of 128 bytes x box_rows.
+static bool make_map(CUtensorMap* m, const void* ptr, uint64_t width, uint64_t rows,
+                     uint64_t pitch, uint32_t box_rows) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return false;
+  cuuint64_t dims[2] = {width, rows};
+  cuuint64_t strides[1] = {pitch};
+  cuuint32_t box[2] = {BK, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box,
+             estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+using Kern = void (*)(const CUtensorMap, const CUtensorMap, const Params);
+static const Kern kPair[2][2] = {
+    {linear_pair_kernel<KIND_I8, false>, linear_pair_kernel<KIND_I8, true>},
+    {linear_pair_kernel<KIND_BF16, false>, linear_pair_kernel<KIND_BF16, true>}};
+static const Kern kStream[2][2] = {
+    {linear_stream_kernel<KIND_I8, false>, linear_stream_kernel<KIND_I8, true>},
+    {linear_stream_kernel<KIND_BF16, false>, linear_stream_kernel<KIND_BF16, true>}};
+
+// Opts the kernels in to the whole shared memory once a device, and asks how many clusters of
+// 1, 2, 4 and 8 streaming CTAs the device holds at once.
+struct DeviceSetup {
+  bool ready = false;
+  int clusters[4] = {0, 0, 0, 0};
+};
+
+static qgemm_status device_setup(qgemm_stream_s* s, const DeviceSetup** out) {
+  static std::mutex mu;
+  static DeviceSetup setup[64];
+  const int ord = s->dev->ordinal;
+  if (ord < 0 || ord >= 64) return fail(QGEMM_ERR_UNSUPPORTED, "device ordinal %d >= 64", ord);
+  std::lock_guard<std::mutex> lock(mu);
+  DeviceSetup& d = setup[ord];
+  if (!d.ready) {
+    for (int k = 0; k < 2; ++k)
+      for (int g = 0; g < 2; ++g) {
+        cudaError_t e = cudaFuncSetAttribute(kPair[k][g], cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
+        if (e == cudaSuccess)
+          e = cudaFuncSetAttribute(kStream[k][g], cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
+        if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(linear)");
+      }
+    for (int i = 0; i < 4; ++i) {
+      const int c = 1 << i;
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(s->dev->sm_count / c * c);
+      cfg.blockDim = dim3(strm::THREADS);
+      cfg.dynamicSmemBytes = SMEM_MAX;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = c;
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      int n = 0;
+      const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kStream[0][0], &cfg);
+      if (e != cudaSuccess) return cuda_fail(e, "cudaOccupancyMaxActiveClusters(linear)");
+      d.clusters[i] = n;
+    }
+    d.ready = true;
+  }
+  *out = &d;
+  return QGEMM_OK;
+}
+
+}  // namespace lin
+
+bool linear_tcgen05_supported(const qgemm_device_s* d, const LinArgs& a, const char** why) {
+  auto no = [&](const char* w) { if (why) *why = w; return false; };
+  const int es = a.kind == KIND_I8 ? 1 : 2;
+  if (!d->tcgen05) return no("device is not sm_100 (tcgen05 unavailable)");
+  if (d->smem_optin < (size_t)lin::SMEM_MAX) return no("not enough shared memory per block");
+  if (a.K <= 0) return no("K == 0");
+  // tiles and rows are counted in 32 bits
+  if (a.M > (1 << 30) || ((long long)a.M / 16 + a.E) * (a.N / 64 + 1) > (1ll << 30))
+    return no("more than 2^30 tiles");
+  if (((long long)a.K * es) % 16 != 0) return no("K is not a multiple of 16 bytes");
+  if ((a.ldx * es) % 16 != 0) return no("the rows of x are not a multiple of 16 bytes apart");
+  if (!aligned((uint64_t)a.x, 16) || !aligned((uint64_t)a.w, 16))
+    return no("x and w must be 16-byte aligned");
+  return true;
+}
+
+qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
+  using namespace lin;
+  const DeviceSetup* ds = nullptr;
+  qgemm_status st = device_setup(s, &ds);
+  if (st != QGEMM_OK) return st;
+  const int es = a.kind == KIND_I8 ? 1 : 2, os = a.out_dtype == QGEMM_F32 ? 4 : 2;
+  const int sms = s->dev->sm_count;
+  Params p = {};
+  p.ep.sx = a.sx; p.ep.sw = a.sw; p.ep.bias = a.bias; p.ep.residual = a.residual;
+  p.ep.out = a.out; p.ep.ldr = a.ldr; p.ep.ldc = a.ldc;
+  p.ep.N = a.N; p.ep.nw = a.gated ? 2 * a.N : a.N;
+  p.ep.out_f32 = a.out_dtype == QGEMM_F32;
+  p.ep.act = a.act;
+  p.ep.vec = aligned((uint64_t)a.out, 4 * os) && a.ldc % 4 == 0 &&
+             (!a.residual || (aligned((uint64_t)a.residual, 4 * os) && a.ldr % 4 == 0));
+  p.offsets = a.offsets;
+  p.E = a.E; p.M = a.M;
+  p.num_k_blocks = (int)(((long long)a.K * es + BK - 1) / BK);
+  p.err = s->dev->d_err;
+  p.wait_ns = s->dev->wait_ns;
+  p.feats = a.gated ? 64 : 128;
+  const int table = ((3 * a.E + 1) * 4 + 15) / 16 * 16;
+  // rows of a group if they are spread evenly; the kernels take any spread
+  const int groups = a.E < a.M ? a.E : a.M;
+  const int avg = (a.M + groups - 1) / groups;
+  const bool use_pair = avg > 128;
+  const int w_rows = a.gated ? 64 : WROWS;  // of a weight box
+  CUtensorMap tmW, tmX;
+  if (!make_map(&tmW, a.w, (uint64_t)a.K * es, (uint64_t)a.E * p.ep.nw, (uint64_t)a.K * es, w_rows))
+    return fail(QGEMM_ERR_CUDA, "cuTensorMapEncodeTiled failed for the weights");
+  cudaLaunchConfig_t cfg = {};
+  cfg.stream = s->stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  Kern kern;
+  int box;
+  if (use_pair) {
+    p.tok_max = pair::TOK;
+    p.tok_round = 32;
+    p.num_w_blocks = (a.N + 2 * p.feats - 1) / (2 * p.feats);
+    box = pair::BOX;
+    const int fixed = pair::STG_BYTES + BAR_BYTES + table + 1024;
+    p.stages = (SMEM_MAX - fixed) / pair::STAGE_BYTES;
+    cfg.dynamicSmemBytes = (size_t)fixed + (size_t)p.stages * pair::STAGE_BYTES;
+    cfg.gridDim = dim3(sms / 2 * 2);
+    cfg.blockDim = dim3(pair::THREADS);
+    kern = kPair[a.kind == KIND_I8 ? 0 : 1][a.gated];
+  } else {
+    // tokens of a tile: twice the even share, so that a moderate skew stays in one tile
+    const int want = a.offsets ? (2 * avg < a.M ? 2 * avg : a.M) : a.M;
+    p.tok_max = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : 128;
+    p.tok_round = 16;
+    p.num_w_blocks = (a.N + p.feats - 1) / p.feats;
+    box = p.tok_max < 32 ? p.tok_max : 32;
+    const int stage = W_BYTES + p.tok_max * BK;
+    const int fixed = p.tok_max * WROWS * 4 + BAR_BYTES + table + 1024;
+    p.stages = (SMEM_MAX - fixed) / stage;
+    if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
+    cfg.dynamicSmemBytes = (size_t)fixed + (size_t)p.stages * stage;
+    // Cut of K: rounds of tiles over the clusters that fit, times the k-blocks of a part,
+    // plus a part's fixed cost (pipeline fill and exchange, about 3 k-blocks' time).
+    const long long tiles = (long long)p.num_w_blocks * ((a.M / p.tok_max) + groups);
+    double best = 0;
+    int pick = 0;
+    for (int i = 0; i < 4; ++i) {
+      const int c = 1 << i;
+      if (ds->clusters[i] < 1 || c > p.num_k_blocks) continue;
+      const long long rounds = (tiles + ds->clusters[i] - 1) / ds->clusters[i];
+      const double cost = (double)rounds * ((p.num_k_blocks + c - 1) / c + (c > 1 ? 3 : 1));
+      if (best == 0 || cost < best) { best = cost; pick = i; }
+    }
+    p.csize = 1 << pick;
+    const long long clusters = tiles < ds->clusters[pick] ? tiles : ds->clusters[pick];
+    cfg.gridDim = dim3((unsigned)(clusters * p.csize));
+    cfg.blockDim = dim3(strm::THREADS);
+    kern = kStream[a.kind == KIND_I8 ? 0 : 1][a.gated];
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = p.csize;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
+  }
+  if (!make_map(&tmX, a.x, (uint64_t)a.K * es, (uint64_t)a.M, (uint64_t)a.ldx * es, box))
+    return fail(QGEMM_ERR_CUDA, "cuTensorMapEncodeTiled failed for x");
+  return cuda_fail(cudaLaunchKernelEx(&cfg, kern, tmW, tmX, p), "linear launch");
+}
+
+}  // namespace qg

@@ -238,6 +238,40 @@ __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
+// As above with release semantics at cluster scope: orders the thread's (and, after a
+// __syncwarp, its warp's) writes to any shared memory of the cluster before the arrival.
+__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
+               : "memory");
+}
+
+// One word to shared memory anywhere in the cluster (an address from map_to_rank).
+__device__ __forceinline__ void st_cluster_u32(uint32_t cluster_addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
+}
+
+// mbar_wait whose success acquires at cluster scope (pairs with
+// mbar_arrive_release_cluster on another CTA of the cluster).
+__device__ __forceinline__ bool mbar_wait_acquire_cluster(uint32_t bar, uint32_t parity,
+                                                          const volatile int* abort,
+                                                          unsigned long long limit_ns) {
+  const unsigned long long t0 = globaltimer();
+  for (uint32_t i = 1;; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if ((i & 63u) == 0) {
+      if (abort && *abort) return false;
+      if (globaltimer() - t0 > limit_ns) return false;
+    }
+  }
+}
 
 // 2-D TMA tile load into this CTA's shared memory for a CTA-pair MMA: completion is
 // counted on `bar_cluster`, an mbarrier that may be in the peer CTA.

@@ -276,6 +276,9 @@ qgemm_status qgemm_stream_sync(qgemm_stream_t s) {
     // a kernel that gave up may have left split-tile counters raised
     if (s->ws) cudaMemsetAsync(s->ws, 0, s->ws_bytes, s->stream);
     cudaStreamSynchronize(s->stream);
+    if (err == DEVERR_BAD_INDEX)
+      return fail(QGEMM_ERR_INVALID_ARG,
+                  "an expert offset or row index read on the device was out of range");
     return fail(QGEMM_ERR_TIMEOUT, "a device-side wait ran out (code %d)", err);
   }
   return QGEMM_OK;

@@ -32,6 +32,11 @@ B_NK = 1
 ALGO_AUTO = 0
 ALGO_TCGEN05 = 1
 ALGO_SIMT = 2
+ACT_NONE = 0
+ACT_RELU = 1
+ACT_GELU = 2
+ACT_GELU_TANH = 3
+ACT_SILU = 4
 PREFILL_FRAG = 1
 PREFILL_ONE_TERM = 2
 
@@ -117,6 +122,18 @@ SIGNATURES = {
     "qgemm_matmul_add_bias_f32": (_S, [_P, _U64, _U64, _U64, _U64, _I, _I, _I]),
     "qgemm_sgemm": (_S, [_P, _U64, _U64, _U64, _I, _I, _I, ctypes.c_float, ctypes.c_float]),
     "qgemm_gemv_f32": (_S, [_P, _U64, _U64, _U64, _I, _I]),
+    "qgemm_linear_bf16_nk": (_S, [_P, _U64, _I, _U64, _U64, _U64, _I, _U64, _I, _I, _I, _I, _I, _I,
+                                  _I, _I]),
+    "qgemm_w8a8_linear": (_S, [_P, _U64, _I, _U64, _U64, _U64, _U64, _U64, _I, _U64, _I, _I, _I,
+                               _I, _I, _I, _I, _I]),
+    "qgemm_expert_linear_bf16_nk": (_S, [_P, _U64, _I, _U64, _U64, _U64, _U64, _I, _I, _I, _I, _I,
+                                         _I, _I, _I, _I]),
+    "qgemm_w8a8_expert_linear": (_S, [_P, _U64, _I, _U64, _U64, _U64, _U64, _U64, _U64, _I, _I,
+                                      _I, _I, _I, _I, _I, _I, _I]),
+    "qgemm_route_topk": (_S, [_P, _U64, _I, _U64, _U64, _U64, _U64, _I, _I, _I, _I]),
+    "qgemm_dispatch_rows": (_S, [_P, _U64, _I, _U64, _U64, _I, _I, _I, _I]),
+    "qgemm_dispatch_rows_quantized": (_S, [_P, _U64, _I, _U64, _U64, _U64, _I, _I, _I, _I]),
+    "qgemm_combine_rows": (_S, [_P, _U64, _I, _U64, _U64, _U64, _U64, _I, _I, _I, _I, _I]),
     "qgemm_prepack_w8_nk": (_S, [_P, _U64, _U64, _I, _I]),
     "qgemm_launch_by_name": (_S, [_P, ctypes.c_char_p, ctypes.POINTER(_U64), _I,
                                   ctypes.POINTER(_I), _I]),

@@ -169,6 +169,78 @@ class QuantizedGemmOps:
         L.call("qgemm_quantize_per_token", self._h, L.addr(x), in_dtype, L.addr(q), L.addr(sA),
                M, K)
 
+    # -- linear layers with their epilogue, dense and grouped by expert ---------
+
+    def linearBf16NK(self, x, w, out, M: int, N: int, K: int, *, bias=None, residual=None,
+                     act: int = L.ACT_NONE, gated: bool = False, out_dtype: int = L.BF16,
+                     ldx: int | None = None, ldr: int | None = None, ldc: int | None = None,
+                     algo: int = L.ALGO_AUTO):
+        """out[M,N] = act(x w^T + bias) + residual: x bf16 [M,K], w bf16 [N,K], bias f32 [N],
+        residual of out_dtype.  gated: w [2N,K] (gate rows, then up rows), bias [2N],
+        out = act(gate) * up + residual."""
+        L.call("qgemm_linear_bf16_nk", self._h, L.addr(x), K if ldx is None else ldx, L.addr(w),
+               L.addr(bias), L.addr(residual), N if ldr is None else ldr, L.addr(out), out_dtype,
+               N if ldc is None else ldc, M, N, K, act, 1 if gated else 0, algo)
+
+    def w8a8Linear(self, A, B, sA, sB, out, M: int, N: int, K: int, *, bias=None, residual=None,
+                   act: int = L.ACT_NONE, gated: bool = False, out_dtype: int = L.BF16,
+                   lda: int | None = None, ldr: int | None = None, ldc: int | None = None,
+                   algo: int = L.ALGO_AUTO):
+        """linearBf16NK on int8 operands: A [M,K], B [N,K] (K-major, see prepackW8NK), per-token
+        sA [M] and per-channel sB [N] ([2N,K] and [2N] when gated)."""
+        L.call("qgemm_w8a8_linear", self._h, L.addr(A), K if lda is None else lda, L.addr(B),
+               L.addr(sA), L.addr(sB), L.addr(bias), L.addr(residual), N if ldr is None else ldr,
+               L.addr(out), out_dtype, N if ldc is None else ldc, M, N, K, act,
+               1 if gated else 0, algo)
+
+    def expertLinearBf16NK(self, x, w, offsets, out, E: int, M: int, N: int, K: int, *, bias=None,
+                           act: int = L.ACT_NONE, gated: bool = False, out_dtype: int = L.BF16,
+                           ldx: int | None = None, ldc: int | None = None,
+                           algo: int = L.ALGO_AUTO):
+        """linearBf16NK with a weight matrix per expert, w [E,N,K] (bias [E,N]): rows
+        offsets[e] .. offsets[e+1] of x go through w[e].  offsets int32 [E+1] on the device
+        (routeTopK makes them); rows of no expert are not written."""
+        L.call("qgemm_expert_linear_bf16_nk", self._h, L.addr(x), K if ldx is None else ldx,
+               L.addr(w), L.addr(bias), L.addr(offsets), L.addr(out), out_dtype,
+               N if ldc is None else ldc, E, M, N, K, act, 1 if gated else 0, algo)
+
+    def w8a8ExpertLinear(self, A, B, sA, sB, offsets, out, E: int, M: int, N: int, K: int, *,
+                         bias=None, act: int = L.ACT_NONE, gated: bool = False,
+                         out_dtype: int = L.BF16, lda: int | None = None,
+                         ldc: int | None = None, algo: int = L.ALGO_AUTO):
+        """w8a8Linear with a weight matrix per expert, B [E,N,K], sB [E,N]; offsets as in
+        expertLinearBf16NK."""
+        L.call("qgemm_w8a8_expert_linear", self._h, L.addr(A), K if lda is None else lda,
+               L.addr(B), L.addr(sA), L.addr(sB), L.addr(bias), L.addr(offsets), L.addr(out),
+               out_dtype, N if ldc is None else ldc, E, M, N, K, act, 1 if gated else 0, algo)
+
+    # -- tokens to experts and back ---------------------------------------------
+
+    def routeTopK(self, logits, weights, experts, offsets, rows, T: int, E: int, k: int, *,
+                  renormalize: bool = True, in_dtype: int = L.F32):
+        """The k largest of E logits of every token (ties to the lower index) with their softmax
+        weights f32 [T,k] and experts int32 [T,k], grouped by expert: offsets int32 [E+1],
+        rows int32 [T,k] (each pair's row in expert order; -1 where nothing is chosen)."""
+        L.call("qgemm_route_topk", self._h, L.addr(logits), in_dtype, L.addr(weights),
+               L.addr(experts), L.addr(offsets), L.addr(rows), T, E, k, 1 if renormalize else 0)
+
+    def dispatchRows(self, x, rows, out, T: int, k: int, K: int, R: int, *, dtype: int = L.BF16):
+        """out[rows[t,j]] = x[t]: x [T,K], out [R,K] of one type."""
+        L.call("qgemm_dispatch_rows", self._h, L.addr(x), dtype, L.addr(rows), L.addr(out), T, k,
+               K, R)
+
+    def dispatchRowsQuantized(self, x, rows, q, sA, T: int, k: int, K: int, R: int, *,
+                              in_dtype: int = L.BF16):
+        """dispatchRows with quantizePerToken on the way: q int8 [R,K], sA f32 [R]."""
+        L.call("qgemm_dispatch_rows_quantized", self._h, L.addr(x), in_dtype, L.addr(rows),
+               L.addr(q), L.addr(sA), T, k, K, R)
+
+    def combineRows(self, y, rows, weights, out, T: int, k: int, N: int, R: int, *, residual=None,
+                    in_dtype: int = L.BF16, out_dtype: int = L.BF16):
+        """out[t] = sum_j weights[t,j] * y[rows[t,j]] (+ residual[t]), fp32 sums."""
+        L.call("qgemm_combine_rows", self._h, L.addr(y), in_dtype, L.addr(rows), L.addr(weights),
+               L.addr(residual), L.addr(out), out_dtype, T, k, N, R)
+
     def prepackW8NK(self, src_kn, dst_nk, K: int, N: int):
         L.call("qgemm_prepack_w8_nk", self._h, L.addr(src_kn), L.addr(dst_nk), K, N)
 

@@ -77,6 +77,17 @@ enum {
   QGEMM_ALGO_SIMT = 2      /* CUDA-core path (any shape), the independent check  */
 };
 
+/* Activations of the linear layers (qgemm_linear_bf16_nk and its siblings).
+ * GELU is 0.5 v (1 + erf(v / sqrt 2)); GELU_TANH its tanh form
+ * 0.5 v (1 + tanh(sqrt(2/pi) (v + 0.044715 v^3))); SILU is v / (1 + exp(-v)). */
+enum {
+  QGEMM_ACT_NONE = 0,
+  QGEMM_ACT_RELU = 1,
+  QGEMM_ACT_GELU = 2,
+  QGEMM_ACT_GELU_TANH = 3,
+  QGEMM_ACT_SILU = 4
+};
+
 typedef struct qgemm_device_s* qgemm_device_t;
 typedef struct qgemm_stream_s* qgemm_stream_t;
 typedef struct qgemm_comm_s* qgemm_comm_t;
@@ -390,6 +401,99 @@ QGEMM_API qgemm_status qgemm_sgemm(qgemm_stream_t s, uint64_t A, uint64_t B, uin
                                    int N, int K, float alpha, float beta);
 QGEMM_API qgemm_status qgemm_gemv_f32(qgemm_stream_t s, uint64_t A, uint64_t x, uint64_t y, int M,
                                       int N);
+
+/* ---- linear layers with their epilogue -------------------------------------
+ * A GEMM with everything up to the next layer in its epilogue (the reference's own fused
+ * form is MatrixOps.matmulAddBias, MatrixOps.scala:31-44, and the hasBias path of
+ * w8a16Gemm, QuantizedGemmOps.scala:24-55):
+ *     z[m,n] = sum_k x[m,k] * w[n,k]                      bf16 operands, fp32 sums
+ *     z[m,n] = (float(sum_k A[m,k] * B[n,k]) * sB[n]) * sA[m]     int8 operands
+ *     y[m,n] = act(z[m,n] + bias[n]) + residual[m,n]
+ * With gated != 0 the weights have 2 N rows, N gate rows and then N up rows (bias and sB
+ * likewise), and  y[m,n] = act(z_gate + bias_gate) * (z_up + bias_up) + residual[m,n].
+ *   x / A     [M, ldx], w / B [N or 2 N, K] (K-major), bf16 or int8
+ *   bias      f32 [N or 2 N], 0 for none
+ *   residual  [M, ldr] of out_dtype, 0 for none; may be `out` itself with ldr == ldc (the
+ *             layer then adds onto the stream in place)
+ *   out       [M, ldc] of out_dtype (QGEMM_BF16 or QGEMM_F32); nothing past column N of a
+ *             row is written
+ * Everything is fp32 up to one rounding (RNE) to out_dtype.  Deterministic: the same call
+ * gives the same bits, whatever ran before.  Nothing is allocated and no scratch is used,
+ * so calls on different streams, and captured graphs, are independent.  QGEMM_ALGO_AUTO
+ * runs on the tensor cores when K is a multiple of 16 bytes and x, w and their rows are
+ * 16-byte aligned, else on CUDA cores (any K >= 0, any ldx; for odd shapes, not fast);
+ * QGEMM_ALGO_TCGEN05 refuses what the tensor cores cannot take (QGEMM_ERR_UNSUPPORTED).
+ * M == 0 or N == 0 does nothing.  int8: K <= 131071 (the int32 sums cannot overflow).
+ * `out` may not overlap x, w, or (unless it is the same buffer) the residual. */
+QGEMM_API qgemm_status qgemm_linear_bf16_nk(qgemm_stream_t s, uint64_t x, int ldx, uint64_t w,
+                                            uint64_t bias, uint64_t residual, int ldr,
+                                            uint64_t out, int out_dtype, int ldc, int M, int N,
+                                            int K, int act, int gated, int algo);
+QGEMM_API qgemm_status qgemm_w8a8_linear(qgemm_stream_t s, uint64_t A, int lda, uint64_t B,
+                                         uint64_t sA, uint64_t sB, uint64_t bias,
+                                         uint64_t residual, int ldr, uint64_t out, int out_dtype,
+                                         int ldc, int M, int N, int K, int act, int gated,
+                                         int algo);
+
+/* The same layer with one weight matrix for each of E experts (1 <= E <= 1024), over rows
+ * sorted by expert: rows offsets[e] <= m < offsets[e + 1] of x go through w[e].
+ *   w / B     [E, N or 2 N, K]; sB, bias f32 [E, N or 2 N]
+ *   offsets   device int32 [E + 1], 0 <= offsets[e] <= offsets[e + 1] <= M, as made by
+ *             qgemm_route_topk; read by the kernel, so the host need not know the counts
+ * M is the number of rows that x and out have; rows outside every expert (past offsets[E])
+ * are not written.  An expert may have no rows.  Offsets that break the rule above name no
+ * rows (that expert is skipped) and the next qgemm_stream_sync reports
+ * QGEMM_ERR_INVALID_ARG. */
+QGEMM_API qgemm_status qgemm_expert_linear_bf16_nk(qgemm_stream_t s, uint64_t x, int ldx,
+                                                   uint64_t w, uint64_t bias, uint64_t offsets,
+                                                   uint64_t out, int out_dtype, int ldc, int E,
+                                                   int M, int N, int K, int act, int gated,
+                                                   int algo);
+QGEMM_API qgemm_status qgemm_w8a8_expert_linear(qgemm_stream_t s, uint64_t A, int lda, uint64_t B,
+                                                uint64_t sA, uint64_t sB, uint64_t bias,
+                                                uint64_t offsets, uint64_t out, int out_dtype,
+                                                int ldc, int E, int M, int N, int K, int act,
+                                                int gated, int algo);
+
+/* ---- tokens to experts and back --------------------------------------------
+ * The steps around the expert layers.  T tokens, k experts each; R = T * k rows.
+ *
+ * qgemm_route_topk: for each token the k experts with the largest logits (a tie goes to
+ * the lower index), in descending order, and their softmax weights: over all E logits, or
+ * over the k chosen ones with renormalize != 0.
+ *   logits   [T, E] f32 or bf16 (in_dtype); 1 <= E <= 1024, 1 <= k <= min(E, 64)
+ *   weights  f32 [T, k]; experts int32 [T, k]
+ *   offsets  int32 [E + 1]: where each expert's rows start when all (token, slot) pairs are
+ *            sorted by expert, tokens in order inside an expert; offsets[E] is the total
+ *   rows     int32 [T, k]: the row of each pair in that order
+ * An expert whose logit is -inf or NaN is never chosen: where fewer than k are left, the
+ * remaining slots get expert -1, row -1 and weight 0 (a row of padding routes nowhere).  A
+ * logit of +inf counts as the largest finite fp32.  Deterministic, no scratch.
+ *
+ * qgemm_dispatch_rows: out[rows[t,j]] = x[t], x [T, K] f32 or bf16 (dtype), out [R, K] of
+ * the same type.  qgemm_dispatch_rows_quantized: the same with every token quantised on
+ * the way, the arithmetic of qgemm_quantize_per_token (bit for bit): q int8 [R, K], sA f32
+ * [R], the A operand and per-token scales of qgemm_w8a8_expert_linear.
+ *
+ * qgemm_combine_rows: out[t] = sum_j weights[t,j] * y[rows[t,j]] (+ residual[t]), y [R, N]
+ * of in_dtype, fp32 sums with j ascending, residual and out [T, N] of out_dtype; weights 0:
+ * all one; residual 0: none (it may be `out` itself).
+ *
+ * rows[t,j] < 0 names no row (nothing is written, nothing added); a row >= R is skipped and
+ * the next qgemm_stream_sync reports QGEMM_ERR_INVALID_ARG.  Two pairs that name one row
+ * leave either's values there.  Outputs may not overlap inputs, but for the residual. */
+QGEMM_API qgemm_status qgemm_route_topk(qgemm_stream_t s, uint64_t logits, int in_dtype,
+                                        uint64_t weights, uint64_t experts, uint64_t offsets,
+                                        uint64_t rows, int T, int E, int k, int renormalize);
+QGEMM_API qgemm_status qgemm_dispatch_rows(qgemm_stream_t s, uint64_t x, int dtype, uint64_t rows,
+                                           uint64_t out, int T, int k, int K, int R);
+QGEMM_API qgemm_status qgemm_dispatch_rows_quantized(qgemm_stream_t s, uint64_t x, int in_dtype,
+                                                     uint64_t rows, uint64_t q, uint64_t sA,
+                                                     int T, int k, int K, int R);
+QGEMM_API qgemm_status qgemm_combine_rows(qgemm_stream_t s, uint64_t y, int in_dtype,
+                                          uint64_t rows, uint64_t weights, uint64_t residual,
+                                          uint64_t out, int out_dtype, int T, int k, int N,
+                                          int R);
 
 /* One-time weight repack: int8 [K,N] (reference layout) -> [N,K] (K-major). */
 QGEMM_API qgemm_status qgemm_prepack_w8_nk(qgemm_stream_t s, uint64_t src_kn, uint64_t dst_nk,

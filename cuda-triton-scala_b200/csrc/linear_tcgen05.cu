@@ -45,8 +45,7 @@ constexpr int BK = 128;         // bytes of K a stage: one 128-byte swizzle row
 constexpr int UMMA_K = 32;      // bytes of K an MMA
 constexpr int WROWS = 128;      // weight rows of a CTA's tile
 constexpr int W_BYTES = WROWS * BK;          // 16 KB
-constexpr int CHUNK = 16;                    // tokens of a staging buffer
-constexpr int CHUNK_BYTES = CHUNK * WROWS * 4;
+constexpr int CHUNK = 16;                    // accumulator columns (tokens) read at a time
 constexpr int SMEM_MAX = 232448;             // 227 KB
 constexpr int BAR_BYTES = 512;
 constexpr int MAX_STAGES = 12;
@@ -59,8 +58,10 @@ struct Params {
   int tok_max;      // tokens of a tile at most
   int tok_round;    // tokens of a tile are a multiple of this (MMA N)
   int num_w_blocks; // weight blocks of an expert
+  int band;         // token blocks of a band of the schedule
   int feats;        // features of a weight block of one CTA: 128, gated 64
   int stages;
+  int seg_kb;       // k-blocks summed in TMEM before the sums move to registers (SEG)
   int csize;        // CTAs of a cluster (stream kernel)
   int* err;
   unsigned long long wait_ns;
@@ -137,6 +138,7 @@ __device__ __forceinline__ Tile tile_of(const Params& p, const Table& tb, int t,
   const int idx = t - tb.pref[e], cnt = tb.cnt[e];
   const int nblk = blocks_of(p, cnt);
   const int blk = (((cnt + nblk - 1) / nblk) + p.tok_round - 1) / p.tok_round * p.tok_round;
+  band = min(band, nblk);
   const int per_band = band * p.num_w_blocks;
   const int b = idx / per_band, in = idx - b * per_band;
   const int rows = min(nblk - b * band, band);
@@ -245,6 +247,130 @@ __device__ __forceinline__ void finish4(const Epi& ep, const Feat<GATED>& f, int
   }
 }
 
+// ---- finishing a chunk of 16 tokens where the accumulator lies ------------------------------
+
+// A lane's weight row: its feature, scale and bias.  Gated: lanes 0-15 of a warp hold the gate
+// rows of 16 features, lanes 16-31 their up rows.
+template <bool GATED>
+struct Lane {
+  int f;
+  float sw, b;
+};
+
+template <int KIND, bool GATED>
+__device__ __forceinline__ Lane<GATED> lane_of(const Epi& ep, int e, int f0, int q, int lane) {
+  Lane<GATED> l;
+  l.f = f0 + (GATED ? q * 16 + lane % 16 : q * 32 + lane);
+  const size_t at = (size_t)e * ep.nw + l.f + (GATED && lane >= 16 ? ep.N : 0);
+  const bool in = l.f < ep.N;
+  l.sw = KIND == KIND_I8 && in ? __ldg(ep.sw + at) : 0.f;
+  l.b = ep.bias && in ? __ldg(ep.bias + at) : 0.f;
+  return l;
+}
+
+// r: 16 accumulator columns (tokens row0 .. row0 + 15, of which `n` exist) of this lane's
+// weight row, valid after `ready`.  Gated, lanes l and l + 16 hold the gate and the up sums
+// of one feature: one shuffle a token pair gives lane l the even token and lane l + 16 the odd
+// one.  bf16 outputs are stored as feature pairs: one shuffle a token pair gives even lanes
+// both features of the first token and odd lanes those of the second, so that a warp's store
+// covers whole 32-byte sectors of two (gated: four) token rows.  Stores go straight to memory:
+// through a staging buffer in shared memory (256-byte runs of a token) the int8 layer at
+// 8192 x 28672 x 4096 took 827 us instead of 790.
+// FULL: all 16 tokens and all of the warp's features exist.
+template <int KIND, bool GATED, int ACT, bool FULL, typename Ready>
+__device__ __forceinline__ void finish_chunk_t(const Epi& ep, const Lane<GATED>& l, int row0, int n,
+                                               int lane, const uint32_t (&r)[16], Ready&& ready) {
+  constexpr int NV = GATED ? 8 : 16;       // values a lane finishes
+  const int hi = GATED ? lane / 16 : 0;    // value i is token (GATED ? 2 i + hi : i)
+  const int fe = l.f & ~1;                 // packed: features fe, fe + 1
+  const int odd = l.f & 1;
+  const bool packed = !ep.out_f32 && ep.vec2;
+  // packed: pair i of this lane is token `first` + `step` i, feature fe
+  const int first = GATED ? 2 * odd + hi : odd;
+  constexpr int step = GATED ? 4 : 2;
+  // fetched while the accumulator load is under way
+  float sx = 0.f;
+  if (KIND == KIND_I8 && (FULL || lane % 16 < n)) sx = __ldg(ep.sx + row0 + lane % 16);
+  float res[NV];
+  if (ep.residual) {
+    if (packed) {
+      const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(ep.residual) +
+                               (size_t)(row0 + first) * ep.ldr + fe;
+#pragma unroll
+      for (int i = 0; i < NV / 2; ++i, p += step * ep.ldr) {
+        uint32_t w = 0;
+        if (FULL || (first + step * i < n && fe + 1 < ep.N)) w = *reinterpret_cast<const uint32_t*>(p);
+        else if (first + step * i < n && fe < ep.N) w = *reinterpret_cast<const uint16_t*>(p);
+        res[2 * i] = __uint_as_float(w << 16);
+        res[2 * i + 1] = __uint_as_float(w & 0xffff0000u);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int t = GATED ? 2 * i + hi : i;
+        res[i] = FULL || (t < n && l.f < ep.N)
+                     ? load_out(ep.residual, ep.out_f32, (size_t)(row0 + t) * ep.ldr + l.f) : 0.f;
+      }
+    }
+  }
+  ready();
+  float v[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const float s = KIND == KIND_I8 ? __shfl_sync(0xffffffffu, sx, j) : 0.f;
+    v[j] = __fadd_rn(dequant<KIND>(r[j], l.sw, s), l.b);
+    if (!GATED) v[j] = activate(ACT, v[j]);
+  }
+  if constexpr (GATED) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float other = __shfl_xor_sync(0xffffffffu, hi ? v[2 * i] : v[2 * i + 1], 16);
+      const float gate = hi ? other : v[2 * i], up = hi ? v[2 * i + 1] : other;
+      v[i] = __fmul_rn(activate(ACT, gate), up);
+    }
+  }
+  if (packed) {
+    __nv_bfloat16* p = static_cast<__nv_bfloat16*>(ep.out) + (size_t)(row0 + first) * ep.ldc + fe;
+#pragma unroll
+    for (int i = 0; i < NV / 2; ++i, p += step * ep.ldc) {
+      uint32_t w;
+      if (ep.residual) {
+        const float other = __shfl_xor_sync(0xffffffffu, odd ? v[2 * i] : v[2 * i + 1], 1);
+        const float a = odd ? other : v[2 * i], b = odd ? v[2 * i + 1] : other;
+        const __nv_bfloat162 h = __floats2bfloat162_rn(__fadd_rn(a, res[2 * i]),
+                                                       __fadd_rn(b, res[2 * i + 1]));
+        w = *reinterpret_cast<const uint32_t*>(&h);
+      } else {  // rounded first, so that one word crosses and one byte permute sorts
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        const uint32_t mine = *reinterpret_cast<const uint32_t*>(&h);
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
+        w = odd ? __byte_perm(other, mine, 0x7632) : __byte_perm(mine, other, 0x5410);
+      }
+      if (FULL || (first + step * i < n && fe + 1 < ep.N)) *reinterpret_cast<uint32_t*>(p) = w;
+      else if (first + step * i < n && fe < ep.N) *reinterpret_cast<uint16_t*>(p) = (uint16_t)w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int t = GATED ? 2 * i + hi : i;
+      if (FULL || (t < n && l.f < ep.N)) {
+        const float y = ep.residual ? __fadd_rn(v[i], res[i]) : v[i];
+        store_out(ep.out, ep.out_f32, (size_t)(row0 + t) * ep.ldc + l.f, y);
+      }
+    }
+  }
+}
+
+template <int KIND, bool GATED, int ACT, typename Ready>
+__device__ __forceinline__ void finish_chunk(const Epi& ep, const Lane<GATED>& l, int row0, int n,
+                                             int lane, const uint32_t (&r)[16], Ready&& ready) {
+  const int last = l.f - (GATED ? lane % 16 - 15 : lane - 31);  // the warp's last feature
+  if (n >= 16 && last < ep.N)
+    finish_chunk_t<KIND, GATED, ACT, true>(ep, l, row0, n, lane, r, ready);
+  else
+    finish_chunk_t<KIND, GATED, ACT, false>(ep, l, row0, n, lane, r, ready);
+}
+
 // Calls fn with the activation as a compile-time constant.
 template <typename F>
 __device__ __forceinline__ void with_act(int act, F&& fn) {
@@ -275,11 +401,11 @@ namespace pair {
 constexpr int TOK = 256;                  // tokens of a tile at most (MMA N)
 constexpr int TOK_BYTES = (TOK / 2) * BK; // each CTA holds half the tokens: 16 KB a stage
 constexpr int STAGE_BYTES = W_BYTES + TOK_BYTES;
-constexpr int BOX = 64;                   // token rows of a TMA box
+constexpr int BOX = 32;                   // token rows of a TMA box where half a tile has
+                                          // fewer than 97 (else one box of 128)
 constexpr int EPI_WARPS = 8;              // two groups of four (one warp a TMEM lane quadrant)
 constexpr int THREADS = 64 + 32 * EPI_WARPS;
-constexpr int STG_BYTES = 2 * 2 * CHUNK_BYTES;  // two buffers for each group
-constexpr int BAND = 8;
+constexpr int SEG_TOK = 128;              // tokens of a tile at most with SEG
 }  // namespace pair
 
 // Item i of pair `pid`: a whole tile in the full rounds; in the last round the `rest` tiles
@@ -290,13 +416,13 @@ __device__ __forceinline__ bool pair_item(const Params& p, const Table& tb, int 
   const int T = tb.pref[p.E];
   const int rounds = T / npairs, rest = T - rounds * npairs;
   if (i < rounds) {
-    r = tile_of(p, tb, pid + i * npairs, pair::BAND);
+    r = tile_of(p, tb, pid + i * npairs, p.band);
     return true;
   }
   if (i > rounds || rest == 0) return false;
   const int parts = min(4, npairs / rest);
   if (pid >= rest * parts) return false;
-  r = tile_of(p, tb, rounds * npairs + pid / parts, pair::BAND);
+  r = tile_of(p, tb, rounds * npairs + pid / parts, p.band);
   if (parts > 1) {
     const int w = ((r.n + parts - 1) / parts + p.tok_round - 1) / p.tok_round * p.tok_round;
     const int first = (pid % parts) * w;
@@ -306,18 +432,19 @@ __device__ __forceinline__ bool pair_item(const Params& p, const Table& tb, int 
   return true;
 }
 
-template <int KIND, bool GATED>
+template <int KIND, bool GATED, bool SEG>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
     linear_pair_kernel(const __grid_constant__ CUtensorMap tmW,
-                       const __grid_constant__ CUtensorMap tmX, const Params p) {
+                       const __grid_constant__ CUtensorMap tmG,
+                       const __grid_constant__ CUtensorMap tmX,
+                       const __grid_constant__ CUtensorMap tmXs, const Params p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_base = ptx::smem_u32(smem_raw);
   const uint32_t base = (raw_base + 1023u) & ~1023u;
   uint8_t* gbase = smem_raw + (base - raw_base);
   const int S = p.stages;
-  const uint32_t stg_base = base + S * pair::STAGE_BYTES;
-  const uint32_t bar_base = stg_base + pair::STG_BYTES;
-  uint8_t* gbar = gbase + S * pair::STAGE_BYTES + pair::STG_BYTES;
+  const uint32_t bar_base = base + S * pair::STAGE_BYTES;
+  uint8_t* gbar = gbase + S * pair::STAGE_BYTES;
   auto full_bar = [&](int s) { return bar_base + 8u * s; };
   auto empty_bar = [&](int s) { return bar_base + 8u * (MAX_STAGES + s); };
   auto tfull_bar = [&](int a) { return bar_base + 8u * (2 * MAX_STAGES + a); };
@@ -372,11 +499,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
       for (int item = 0; ok && pair_item(p, tb, pid, npairs, item, it_); ++item) {
         if (it_.n == 0) continue;
         const int half = (it_.n + p.tok_round - 1) / p.tok_round * p.tok_round / 2;
-        const int boxes = (half + pair::BOX - 1) / pair::BOX;
+        const int boxes = (half + pair::BOX - 1) / pair::BOX;  // 1 to 4
         const uint32_t tx = 2u * (W_BYTES + (uint32_t)boxes * pair::BOX * BK);
         const int x0 = it_.t0 + (int)rank * half;
         // this CTA's weight rows: 128 of the block's 256, or 64 gate and 64 up rows
-        const int w0 = it_.e * p.ep.nw + (it_.wb * 2 + (int)rank) * p.feats;
+        const int f0 = (it_.wb * 2 + (int)rank) * p.feats;
+        const int w0 = it_.e * p.ep.nw + f0;
         for (int kb = 0; kb < p.num_k_blocks; ++kb) {
           if (!ptx::mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.wait_ns)) {
             if (!*abort_flag) report_cluster(p.err, DEVERR_TIMEOUT_PRODUCER, abort_flag, 2);
@@ -386,10 +514,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
           const uint32_t sw = base + stage * pair::STAGE_BYTES, sx = sw + W_BYTES;
           const uint32_t fb = ptx::map_to_rank(full_bar(stage), 0);
           if (rank == 0) ptx::mbar_arrive_expect_tx(full_bar(stage), tx);
-          ptx::tma_load_2d_pair(sw, &tmW, fb, kb * BK, w0);
-          if (GATED) ptx::tma_load_2d_pair(sw + W_BYTES / 2, &tmW, fb, kb * BK, w0 + p.ep.N);
-          for (int b = 0; b < boxes; ++b)
-            ptx::tma_load_2d_pair(sx + b * pair::BOX * BK, &tmX, fb, kb * BK, x0 + b * pair::BOX);
+          if constexpr (GATED) {
+            // 16 gate rows, the 16 up rows of the same features, and so on: both halves of
+            // a feature's product land in one warp's TMEM lanes.  One copy through the 5-D
+            // map (k, row of 16, gate / up, block of 16 features, expert) where all 64
+            // features lie in whole blocks, else eight (the last features of an N that is
+            // not a multiple of 16; eight copies for every tile made the layer 25 % slower)
+            if (f0 + 64 <= p.ep.N / 16 * 16) {
+              ptx::tma_load_5d_pair(sw, &tmG, fb, kb * BK, 0, 0, f0 / 16, it_.e);
+            } else
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+              ptx::tma_load_2d_pair(sw + (2 * b) * 16 * BK, &tmW, fb, kb * BK, w0 + 16 * b);
+              ptx::tma_load_2d_pair(sw + (2 * b + 1) * 16 * BK, &tmW, fb, kb * BK,
+                                    w0 + p.ep.N + 16 * b);
+            }
+          } else {
+            ptx::tma_load_2d_pair(sw, &tmW, fb, kb * BK, w0);
+          }
+          if (boxes == 4)
+            ptx::tma_load_2d_pair(sx, &tmX, fb, kb * BK, x0);
+          else
+            for (int b = 0; b < boxes; ++b)
+              ptx::tma_load_2d_pair(sx + b * pair::BOX * BK, &tmXs, fb, kb * BK, x0 + b * pair::BOX);
           ++issued;
           if (++stage == S) { stage = 0; phase ^= 1u; }
         }
@@ -416,36 +563,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
         const int ncol = (it_.n + p.tok_round - 1) / p.tok_round * p.tok_round;
         const uint32_t idesc = KIND == KIND_BF16 ? ptx::idesc_bf16(256, ncol)
                                                  : ptx::idesc_i8(256, ncol, false, false);
-        const int a = it & 1;
-        if (!ptx::mbar_wait(tempty_bar(a), (uint32_t)((it >> 1) & 1) ^ 1u, abort_flag, p.wait_ns)) {
-          if (!*abort_flag) report_cluster(p.err, DEVERR_TIMEOUT_MMA, abort_flag, 2);
-          ok = false;
-          break;
-        }
-        ++it;
-        ptx::tc_fence_after();
-        const uint32_t d_tmem = tmem_base + (uint32_t)(a * 256);
-        for (int kb = 0; kb < p.num_k_blocks; ++kb) {
-          if (!ptx::mbar_wait(full_bar(stage), phase, abort_flag, p.wait_ns)) {
+        const int seg = SEG ? p.seg_kb : p.num_k_blocks;
+        for (int kb0 = 0; ok && kb0 < p.num_k_blocks; kb0 += seg) {
+          const int a = it & 1;
+          if (!ptx::mbar_wait(tempty_bar(a), (uint32_t)((it >> 1) & 1) ^ 1u, abort_flag, p.wait_ns)) {
             if (!*abort_flag) report_cluster(p.err, DEVERR_TIMEOUT_MMA, abort_flag, 2);
             ok = false;
             break;
           }
+          ++it;
           ptx::tc_fence_after();
-          const uint32_t sw = base + stage * pair::STAGE_BYTES, sx = sw + W_BYTES;
+          const uint32_t d_tmem = tmem_base + (uint32_t)(a * 256);
+          const int kb1 = min(kb0 + seg, p.num_k_blocks);
+          for (int kb = kb0; kb < kb1; ++kb) {
+            if (!ptx::mbar_wait(full_bar(stage), phase, abort_flag, p.wait_ns)) {
+              if (!*abort_flag) report_cluster(p.err, DEVERR_TIMEOUT_MMA, abort_flag, 2);
+              ok = false;
+              break;
+            }
+            ptx::tc_fence_after();
+            const uint32_t sw = base + stage * pair::STAGE_BYTES, sx = sw + W_BYTES;
+            const uint32_t empty = empty_bar(stage);
+            if (++stage == S) { stage = 0; phase ^= 1u; }
 #pragma unroll
-          for (int kk = 0; kk < BK / UMMA_K; ++kk) {
-            const uint64_t adesc = ptx::smem_desc_sw128(sw + kk * UMMA_K, 16, 1024);
-            const uint64_t bdesc = ptx::smem_desc_sw128(sx + kk * UMMA_K, 16, 1024);
-            const uint32_t accum = (kb | kk) != 0 ? 1u : 0u;
-            if constexpr (KIND == KIND_BF16) ptx::umma_bf16_pair(d_tmem, adesc, bdesc, idesc, accum);
-            else ptx::umma_i8_pair(d_tmem, adesc, bdesc, idesc, accum);
+            for (int kk = 0; kk < BK / UMMA_K; ++kk) {
+              const uint64_t adesc = ptx::smem_desc_sw128(sw + kk * UMMA_K, 16, 1024);
+              const uint64_t bdesc = ptx::smem_desc_sw128(sx + kk * UMMA_K, 16, 1024);
+              const uint32_t accum = (kb != kb0 || kk != 0) ? 1u : 0u;
+              if constexpr (KIND == KIND_BF16) ptx::umma_bf16_pair(d_tmem, adesc, bdesc, idesc, accum);
+              else ptx::umma_i8_pair(d_tmem, adesc, bdesc, idesc, accum);
+            }
+            ptx::umma_commit_pair(empty, 0x3);
+            issued_any = true;
           }
-          ptx::umma_commit_pair(empty_bar(stage), 0x3);
-          issued_any = true;
-          if (++stage == S) { stage = 0; phase ^= 1u; }
+          if (ok) ptx::umma_commit_pair(tfull_bar(a), 0x3);
         }
-        if (ok) ptx::umma_commit_pair(tfull_bar(a), 0x3);
       }
       if (!ok && issued_any) {
         ptx::umma_commit_pair(drain_bar, 0x1);
@@ -455,86 +607,80 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
     }
   } else {
     // ---------------- epilogue (both CTAs, two groups of four warps) ----------------
-    const int q = warp & 3;             // TMEM lane quadrant: features 32 q ..
+    const int q = warp & 3;             // TMEM lane quadrant
     const int grp = (warp - 2) / 4;     // chunks c with c % 2 == grp
-    const int w4 = (warp - 2) % 4;      // warp of the group
-    const uint32_t stg = stg_base + (uint32_t)grp * 2 * CHUNK_BYTES;
     const uint32_t te0 = ptx::map_to_rank(tempty_bar(0), 0);
     const uint32_t te1 = ptx::map_to_rank(tempty_bar(1), 0);
-    const Epi& ep = p.ep;
-    int it = 0, seq = 0;
+    const uint32_t tmem_q = tmem_base + ((uint32_t)(q * 32) << 16);
+    int it = 0;
     for (int item = 0; pair_item(p, tb, pid, npairs, item, it_); ++item) {
       if (it_.n == 0) continue;
-      const int a = it & 1;
-      const int nf = (it_.wb * 2 + (int)rank) * p.feats + 4 * (GATED ? lane % 16 : lane);
-      Feat<GATED> f;
-      load_feat<KIND, GATED>(ep, it_.e, nf, f);
-      // a warp whose wait ran out keeps the group's barrier sequence and stores nothing
-      bool ok = ptx::mbar_wait_sleep(tfull_bar(a), (uint32_t)((it >> 1) & 1), abort_flag, p.wait_ns);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok && lane == 0 && !*abort_flag)
-        report_cluster(p.err, DEVERR_TIMEOUT_EPILOGUE, abort_flag, 2);
-      ++it;
-      ptx::tc_fence_after();
+      const Lane<GATED> f =
+          lane_of<KIND, GATED>(p.ep, it_.e, (it_.wb * 2 + (int)rank) * p.feats, q, lane);
       const int chunks = (it_.n + CHUNK - 1) / CHUNK;
-      with_act(ep.act, [&](auto act) {
-        for (int c = grp; c < chunks; c += 2, ++seq) {
-          const uint32_t buf = stg + (uint32_t)(seq & 1) * CHUNK_BYTES;
-          uint32_t r[16];
-          if (ok) {
-            ptx::tmem_ld_32x32b_x16(
-                tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * 256 + c * CHUNK), r);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) r[j] = 0u;
-          }
-          // the rows this lane finishes: scales and residuals, while the load is under way
-          constexpr int ROWS = GATED ? 2 : 4;
-          float sx[ROWS], res[ROWS][4];
-          int row[ROWS];
-#pragma unroll
-          for (int i = 0; i < ROWS; ++i) {
-            const int t = GATED ? w4 * 2 + lane / 16 + 8 * i : w4 + 4 * i;
-            const bool in = ok && c * CHUNK + t < it_.n && f.n < ep.N;
-            row[i] = in ? it_.t0 + c * CHUNK + t : -1;
-            sx[i] = 1.f;
-            if (in) {
-              if (KIND == KIND_I8) sx[i] = __ldg(ep.sx + row[i]);
-              load_residual(ep, row[i], f.n, res[i]);
-            }
-          }
-          ptx::tmem_wait_ld();
-          if (c + 2 >= chunks) {  // this warp has read its last columns of the accumulator
-            ptx::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive_remote(a ? te1 : te0);
-          }
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            st_shared_u32(buf + (uint32_t)(j * WROWS + q * 32 + lane) * 4u, r[j]);
-          // one barrier a chunk: the buffer written next is the other one, which every warp
-          // of the group has finished reading before it arrives here
-          ptx::named_bar_sync(1 + grp, 128);
-#pragma unroll
-          for (int i = 0; i < ROWS; ++i) {
-            const int t = GATED ? w4 * 2 + lane / 16 + 8 * i : w4 + 4 * i;
-            const uint32_t at = buf + (uint32_t)(t * WROWS + 4 * (GATED ? lane % 16 : lane)) * 4u;
-            const uint4 gv = ld_shared_v4(at);
-            const uint32_t g[4] = {gv.x, gv.y, gv.z, gv.w};
-            uint32_t u[4] = {0u, 0u, 0u, 0u};
-            if (GATED) {
-              const uint4 uv = ld_shared_v4(at + 64 * 4);
-              u[0] = uv.x; u[1] = uv.y; u[2] = uv.z; u[3] = uv.w;
-            }
-            if (row[i] >= 0)
-              finish4<KIND, GATED, decltype(act)::value>(ep, f, row[i], sx[i], g, u, res[i]);
-          }
-        }
-      });
-      if (grp >= chunks) {  // no chunk of this tile is this group's
+      // Waits for accumulator it & 1; a warp whose wait ran out stores nothing.
+      auto acc_ready = [&]() {
+        bool ok = ptx::mbar_wait_sleep(tfull_bar(it & 1), (uint32_t)((it >> 1) & 1), abort_flag,
+                                       p.wait_ns);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok && lane == 0 && !*abort_flag)
+          report_cluster(p.err, DEVERR_TIMEOUT_EPILOGUE, abort_flag, 2);
+        ptx::tc_fence_after();
+        return ok;
+      };
+      auto acc_done = [&]() {  // this warp has read its columns
         ptx::tc_fence_before();
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive_remote(a ? te1 : te0);
+        if (lane == 0) ptx::mbar_arrive_remote((it & 1) ? te1 : te0);
+        ++it;
+      };
+      if constexpr (!SEG) {
+        const bool ok = acc_ready();
+        const uint32_t acc = tmem_q + (uint32_t)((it & 1) * 256);
+        if (ok)
+          with_act(p.ep.act, [&](auto act) {
+            for (int c = grp; c < chunks; c += 2) {
+              uint32_t r[16];
+              ptx::tmem_ld_32x32b_x16(acc + (uint32_t)(c * CHUNK), r);
+              finish_chunk<KIND, GATED, decltype(act)::value>(
+                  p.ep, f, it_.t0 + c * CHUNK, it_.n - c * CHUNK, lane, r, [] { ptx::tmem_wait_ld(); });
+            }
+          });
+        acc_done();
+      } else {
+        constexpr int MINE = pair::SEG_TOK / CHUNK / 2;  // chunks of a group
+        float run[MINE][16];
+        bool ok = true;
+        for (int kb = 0; kb < p.num_k_blocks; kb += p.seg_kb) {
+          ok = acc_ready() && ok;
+          const uint32_t acc = tmem_q + (uint32_t)((it & 1) * 256);
+#pragma unroll
+          for (int i = 0; i < MINE; ++i) {
+            const int c = grp + 2 * i;
+            if (ok && c < chunks) {
+              uint32_t r[16];
+              ptx::tmem_ld_32x32b_x16(acc + (uint32_t)(c * CHUNK), r);
+              ptx::tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                run[i][j] = kb == 0 ? __uint_as_float(r[j]) : __fadd_rn(run[i][j], __uint_as_float(r[j]));
+            }
+          }
+          acc_done();
+        }
+        if (ok)
+          with_act(p.ep.act, [&](auto act) {
+#pragma unroll
+            for (int i = 0; i < MINE; ++i) {
+              const int c = grp + 2 * i;
+              if (c >= chunks) continue;
+              uint32_t r[16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(run[i][j]);
+              finish_chunk<KIND, GATED, decltype(act)::value>(
+                  p.ep, f, it_.t0 + c * CHUNK, it_.n - c * CHUNK, lane, r, [] {});
+            }
+          });
       }
     }
   }
@@ -552,13 +698,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
 // ---- the streaming kernel ------------------------------------------------------------------
 namespace strm {  // tiles of 16, 32, 64 or 128 tokens at most (Params::tok_max)
 constexpr int THREADS = 192;   // producer, MMA issuer, four epilogue warps
-constexpr int BAND = 1 << 20;  // token blocks run fastest: neighbours share the weights
+constexpr int SEG_TOK = 64;    // tokens of a tile at most with SEG
 }  // namespace strm
 
-template <int KIND, bool GATED>
+template <int KIND, bool GATED, bool SEG>
 __global__ void __launch_bounds__(strm::THREADS, 1)
     linear_stream_kernel(const __grid_constant__ CUtensorMap tmW,
-                         const __grid_constant__ CUtensorMap tmX, const Params p) {
+                         const __grid_constant__ CUtensorMap, const __grid_constant__ CUtensorMap tmX,
+                         const __grid_constant__ CUtensorMap, const Params p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_base = ptx::smem_u32(smem_raw);
   const uint32_t base = (raw_base + 1023u) & ~1023u;
@@ -629,7 +776,7 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
       long long issued = 0;
       bool ok = true;
       for (int tile = cid; ok && tile < T; tile += nclusters) {
-        const Tile t = tile_of(p, tb, tile, strm::BAND);
+        const Tile t = tile_of(p, tb, tile, p.band);
         if (t.n == 0) continue;
         const int boxes = (t.n + box - 1) / box;
         const uint32_t tx = W_BYTES + (uint32_t)(boxes * box * BK);
@@ -665,41 +812,45 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
       int it = 0;
       bool ok = true, issued_any = false;
       for (int tile = cid; ok && tile < T; tile += nclusters) {
-        const Tile t = tile_of(p, tb, tile, strm::BAND);
+        const Tile t = tile_of(p, tb, tile, p.band);
         if (t.n == 0) continue;
         const int ncol = (t.n + 15) / 16 * 16;
         const uint32_t idesc = KIND == KIND_BF16 ? ptx::idesc_bf16(128, ncol)
                                                  : ptx::idesc_i8(128, ncol, false, false);
-        const int a = it & 1;
-        if (!ptx::mbar_wait(tempty_bar(a), (uint32_t)((it >> 1) & 1) ^ 1u, abort_flag, p.wait_ns)) {
-          if (!*abort_flag) report_cluster(p.err, DEVERR_TIMEOUT_MMA, abort_flag, C);
-          ok = false;
-          break;
-        }
-        ++it;
-        ptx::tc_fence_after();
-        const uint32_t d_tmem = tmem_base + (uint32_t)(a * TOK);
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (!ptx::mbar_wait(full_bar(stage), phase, abort_flag, p.wait_ns)) {
+        const int seg = SEG ? p.seg_kb : p.num_k_blocks;
+        for (int s0 = kb0; ok && s0 < kb1; s0 += seg) {
+          const int a = it & 1;
+          if (!ptx::mbar_wait(tempty_bar(a), (uint32_t)((it >> 1) & 1) ^ 1u, abort_flag, p.wait_ns)) {
             if (!*abort_flag) report_cluster(p.err, DEVERR_TIMEOUT_MMA, abort_flag, C);
             ok = false;
             break;
           }
+          ++it;
           ptx::tc_fence_after();
-          const uint32_t sw = base + stage * stage_bytes, sx = sw + W_BYTES;
+          const uint32_t d_tmem = tmem_base + (uint32_t)(a * TOK);
+          const int s1 = min(s0 + seg, kb1);
+          for (int kb = s0; kb < s1; ++kb) {
+            if (!ptx::mbar_wait(full_bar(stage), phase, abort_flag, p.wait_ns)) {
+              if (!*abort_flag) report_cluster(p.err, DEVERR_TIMEOUT_MMA, abort_flag, C);
+              ok = false;
+              break;
+            }
+            ptx::tc_fence_after();
+            const uint32_t sw = base + stage * stage_bytes, sx = sw + W_BYTES;
 #pragma unroll
-          for (int kk = 0; kk < BK / UMMA_K; ++kk) {
-            const uint64_t adesc = ptx::smem_desc_sw128(sw + kk * UMMA_K, 16, 1024);
-            const uint64_t bdesc = ptx::smem_desc_sw128(sx + kk * UMMA_K, 16, 1024);
-            const uint32_t accum = (kb != kb0 || kk != 0) ? 1u : 0u;
-            if constexpr (KIND == KIND_BF16) ptx::umma_bf16(d_tmem, adesc, bdesc, idesc, accum);
-            else ptx::umma_i8(d_tmem, adesc, bdesc, idesc, accum);
+            for (int kk = 0; kk < BK / UMMA_K; ++kk) {
+              const uint64_t adesc = ptx::smem_desc_sw128(sw + kk * UMMA_K, 16, 1024);
+              const uint64_t bdesc = ptx::smem_desc_sw128(sx + kk * UMMA_K, 16, 1024);
+              const uint32_t accum = (kb != s0 || kk != 0) ? 1u : 0u;
+              if constexpr (KIND == KIND_BF16) ptx::umma_bf16(d_tmem, adesc, bdesc, idesc, accum);
+              else ptx::umma_i8(d_tmem, adesc, bdesc, idesc, accum);
+            }
+            ptx::umma_commit(empty_bar(stage));
+            issued_any = true;
+            if (++stage == S) { stage = 0; phase ^= 1u; }
           }
-          ptx::umma_commit(empty_bar(stage));
-          issued_any = true;
-          if (++stage == S) { stage = 0; phase ^= 1u; }
+          if (ok) ptx::umma_commit(tfull_bar(a));
         }
-        if (ok) ptx::umma_commit(tfull_bar(a));
       }
       if (!ok && issued_any) {
         ptx::umma_commit(drain_bar);
@@ -712,34 +863,23 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
     const int q = warp & 3;
     const Epi& ep = p.ep;
     const int slot = TOK / C;  // tokens of a rank's slice at most
-    int it = 0;
+    int it = 0, tiles = 0;
     bool ok = true;
     for (int tile = cid; ok && tile < T; tile += nclusters) {
-      const Tile t = tile_of(p, tb, tile, strm::BAND);
+      const Tile t = tile_of(p, tb, tile, p.band);
       if (t.n == 0) continue;
-      const int a = it & 1;
-      const uint32_t xphase = (uint32_t)(it & 1);  // of the exchange barriers, one use a tile
-      const int per = (t.n + C - 1) / C;           // rank r finishes tokens r * per ..
+      const uint32_t xphase = (uint32_t)(tiles & 1);  // of the exchange barriers, one use a tile
+      ++tiles;
+      const int per = (t.n + C - 1) / C;              // rank r finishes tokens r * per ..
       const int nf = t.wb * p.feats + 4 * (GATED ? lane % 16 : lane);
       Feat<GATED> f;
       load_feat<KIND, GATED>(ep, t.e, nf, f);
-      ok = ptx::mbar_wait(tfull_bar(a), (uint32_t)((it >> 1) & 1), abort_flag, p.wait_ns);
-      ++it;
-      // every rank has read the partial sums of the tile before
-      ok = ok && ptx::mbar_wait_acquire_cluster(rempty_bar, xphase ^ 1u, abort_flag, p.wait_ns);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) {
-        if (lane == 0 && !*abort_flag) report_cluster(p.err, DEVERR_TIMEOUT_EPILOGUE, abort_flag, C);
-        break;
-      }
-      ptx::tc_fence_after();
-      // push each token's 32 sums of this warp to the rank that finishes the token
+      const uint32_t tmem_q = tmem_base + ((uint32_t)(q * 32) << 16);
+      const uint32_t to0 = recv + (uint32_t)((rank * slot) * WROWS + q * 32 + lane) * 4u;
       int dst = 0, tl = 0;
-      uint32_t to = ptx::map_to_rank(recv, 0) + (uint32_t)((rank * slot) * WROWS + q * 32 + lane) * 4u;
-      for (int c = 0; c < t.n; c += 16) {
-        uint32_t r[16];
-        ptx::tmem_ld_32x32b_x16(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * TOK + c), r);
-        ptx::tmem_wait_ld();
+      uint32_t to = ptx::map_to_rank(to0, 0);
+      // pushes 16 tokens' sums of this lane's weight row to the ranks that finish them
+      auto push = [&](int c, const uint32_t (&r)[16]) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           if (c + j < t.n) {
@@ -747,17 +887,59 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
             to += WROWS * 4u;
             if (++tl == per) {
               tl = 0;
-              ++dst;
-              if (dst < C)
-                to = ptx::map_to_rank(recv, dst) +
-                     (uint32_t)((rank * slot) * WROWS + q * 32 + lane) * 4u;
+              if (++dst < C) to = ptx::map_to_rank(to0, dst);
             }
           }
         }
+      };
+      float run[SEG ? strm::SEG_TOK / 16 : 1][16];
+      const int seg = SEG ? p.seg_kb : p.num_k_blocks;
+      for (int s0 = kb0; ok && s0 < kb1; s0 += seg, ++it) {
+        const int a = it & 1;
+        ok = ptx::mbar_wait(tfull_bar(a), (uint32_t)((it >> 1) & 1), abort_flag, p.wait_ns);
+        if (s0 + seg >= kb1)  // every rank has read the partial sums of the tile before
+          ok = ok && ptx::mbar_wait_acquire_cluster(rempty_bar, xphase ^ 1u, abort_flag, p.wait_ns);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        if constexpr (!SEG) {
+          for (int c = 0; c < t.n; c += 16) {
+            uint32_t r[16];
+            ptx::tmem_ld_32x32b_x16(tmem_q + (uint32_t)(a * TOK + c), r);
+            ptx::tmem_wait_ld();
+            push(c, r);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < strm::SEG_TOK / 16; ++i)
+            if (16 * i < t.n) {
+              uint32_t r[16];
+              ptx::tmem_ld_32x32b_x16(tmem_q + (uint32_t)(a * TOK + 16 * i), r);
+              ptx::tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                run[i][j] = s0 == kb0 ? __uint_as_float(r[j]) : __fadd_rn(run[i][j], __uint_as_float(r[j]));
+            }
+        }
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(tempty_bar(a));
       }
-      ptx::tc_fence_before();
+      if (!ok) {
+        if (lane == 0 && !*abort_flag) report_cluster(p.err, DEVERR_TIMEOUT_EPILOGUE, abort_flag, C);
+        break;
+      }
+      if constexpr (SEG) {
+#pragma unroll
+        for (int i = 0; i < strm::SEG_TOK / 16; ++i)
+          if (16 * i < t.n) {
+            uint32_t r[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(run[i][j]);
+            push(16 * i, r);
+          }
+      }
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(tempty_bar(a));
       if (lane < C) ptx::mbar_arrive_release_cluster(ptx::map_to_rank(rfull_bar, lane));
       ok = ptx::mbar_wait_acquire_cluster(rfull_bar, xphase, abort_flag, p.wait_ns);
       ok = __all_sync(0xffffffffu, ok);
@@ -846,13 +1028,39 @@ static bool make_map(CUtensorMap* m, const void* ptr, uint64_t width, uint64_t r
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-using Kern = void (*)(const CUtensorMap, const CUtensorMap, const Params);
-static const Kern kPair[2][2] = {
-    {linear_pair_kernel<KIND_I8, false>, linear_pair_kernel<KIND_I8, true>},
-    {linear_pair_kernel<KIND_BF16, false>, linear_pair_kernel<KIND_BF16, true>}};
-static const Kern kStream[2][2] = {
-    {linear_stream_kernel<KIND_I8, false>, linear_stream_kernel<KIND_I8, true>},
-    {linear_stream_kernel<KIND_BF16, false>, linear_stream_kernel<KIND_BF16, true>}};
+// The gated weights [E][2][N][K] as (k, row of 16, gate / up, block of 16 features, expert);
+// features past the last whole block are outside the map.  Boxes of 128 bytes x 16 rows x both
+// halves x 4 blocks: 128 weight rows, gate and up interleaved by 16.
+static bool make_gated_map(CUtensorMap* m, const void* ptr, uint64_t width, int N, int E) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return false;
+  cuuint64_t dims[5] = {width, 16, 2, (cuuint64_t)(N / 16), (cuuint64_t)E};
+  cuuint64_t strides[4] = {width, (cuuint64_t)N * width, 16 * width, 2 * (cuuint64_t)N * width};
+  cuuint32_t box[5] = {BK, 16, 2, 4, 1};
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, const_cast<void*>(ptr), dims, strides, box,
+             estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+using Kern = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const CUtensorMap,
+                      const Params);
+// [int8, bf16, bf16 in segments][gated]
+static const Kern kPair[3][2] = {
+    {linear_pair_kernel<KIND_I8, false, false>, linear_pair_kernel<KIND_I8, true, false>},
+    {linear_pair_kernel<KIND_BF16, false, false>, linear_pair_kernel<KIND_BF16, true, false>},
+    {linear_pair_kernel<KIND_BF16, false, true>, linear_pair_kernel<KIND_BF16, true, true>}};
+static const Kern kStream[3][2] = {
+    {linear_stream_kernel<KIND_I8, false, false>, linear_stream_kernel<KIND_I8, true, false>},
+    {linear_stream_kernel<KIND_BF16, false, false>, linear_stream_kernel<KIND_BF16, true, false>},
+    {linear_stream_kernel<KIND_BF16, false, true>, linear_stream_kernel<KIND_BF16, true, true>}};
+
+// The tensor cores add each MMA's products to the fp32 accumulator by truncation, so a sum
+// over K shrinks by about 9e-10 of itself a value of K (measured: 2.1e-6 at K = 2048, 1.2e-5 at
+// 11008).  bf16 outputs round 300 times coarser; fp32 outputs take the SEG kernels, which move
+// the accumulator to registers every SEG_KB k-blocks (512 values, 4.7e-7) and add the pieces
+// rounding to nearest.
+constexpr int SEG_KB = 8;
 
 // Opts the kernels in to the whole shared memory once a device, and asks how many clusters of
 // 1, 2, 4 and 8 streaming CTAs the device holds at once.
@@ -869,7 +1077,7 @@ static qgemm_status device_setup(qgemm_stream_s* s, const DeviceSetup** out) {
   std::lock_guard<std::mutex> lock(mu);
   DeviceSetup& d = setup[ord];
   if (!d.ready) {
-    for (int k = 0; k < 2; ++k)
+    for (int k = 0; k < 3; ++k)
       for (int g = 0; g < 2; ++g) {
         cudaError_t e = cudaFuncSetAttribute(kPair[k][g], cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
         if (e == cudaSuccess)
@@ -933,6 +1141,8 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
   p.ep.act = a.act;
   p.ep.vec = aligned((uint64_t)a.out, 4 * os) && a.ldc % 4 == 0 &&
              (!a.residual || (aligned((uint64_t)a.residual, 4 * os) && a.ldr % 4 == 0));
+  p.ep.vec2 = a.out_dtype == QGEMM_BF16 && aligned((uint64_t)a.out, 4) && a.ldc % 2 == 0 &&
+              (!a.residual || (aligned((uint64_t)a.residual, 4) && a.ldr % 2 == 0));
   p.offsets = a.offsets;
   p.E = a.E; p.M = a.M;
   p.num_k_blocks = (int)(((long long)a.K * es + BK - 1) / BK);
@@ -944,8 +1154,15 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
   const int groups = a.E < a.M ? a.E : a.M;
   const int avg = (a.M + groups - 1) / groups;
   const bool use_pair = avg > 128;
-  const int w_rows = a.gated ? 64 : WROWS;  // of a weight box
-  CUtensorMap tmW, tmX;
+  // rows of a weight box: all of a CTA's, or one of its gate or up runs
+  const int w_rows = !a.gated ? WROWS : use_pair ? 16 : 64;
+  p.seg_kb = SEG_KB;
+  const bool seg = a.kind == KIND_BF16 && a.out_dtype == QGEMM_F32 && p.num_k_blocks > SEG_KB;
+  const int variant = a.kind == KIND_I8 ? 0 : seg ? 2 : 1;
+  CUtensorMap tmW, tmG, tmX;
+  memset(&tmG, 0, sizeof(tmG));
+  if (a.gated && use_pair && a.N >= 64 && !make_gated_map(&tmG, a.w, (uint64_t)a.K * es, a.N, a.E))
+    return fail(QGEMM_ERR_CUDA, "cuTensorMapEncodeTiled failed for the gated weights");
   if (!make_map(&tmW, a.w, (uint64_t)a.K * es, (uint64_t)a.E * p.ep.nw, (uint64_t)a.K * es, w_rows))
     return fail(QGEMM_ERR_CUDA, "cuTensorMapEncodeTiled failed for the weights");
   cudaLaunchConfig_t cfg = {};
@@ -958,21 +1175,28 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
   Kern kern;
   int box;
   if (use_pair) {
-    p.tok_max = pair::TOK;
+    p.tok_max = seg ? pair::SEG_TOK : pair::TOK;
+    // A band's tokens stay in L2 while all weights pass by once: the fewer bands, the fewer
+    // times the weights come from HBM, whose power the tensor cores then lack (int8 8192 x
+    // 28672 x 4096: 805 us with 32 MB of tokens a band, 815 with 16, 825 with 8; bf16 4096 x
+    // 4096 x 11008: 318 us with 45 MB, 327 with 90 or 22).
+    const long long block_bytes = (long long)p.tok_max * a.K * es;
+    p.band = (int)(block_bytes > (48 << 20) ? 1 : (48 << 20) / block_bytes);
     p.tok_round = 32;
     p.num_w_blocks = (a.N + 2 * p.feats - 1) / (2 * p.feats);
-    box = pair::BOX;
-    const int fixed = pair::STG_BYTES + BAR_BYTES + table + 1024;
+    box = 128;
+    const int fixed = BAR_BYTES + table + 1024;
     p.stages = (SMEM_MAX - fixed) / pair::STAGE_BYTES;
     cfg.dynamicSmemBytes = (size_t)fixed + (size_t)p.stages * pair::STAGE_BYTES;
     cfg.gridDim = dim3(sms / 2 * 2);
     cfg.blockDim = dim3(pair::THREADS);
-    kern = kPair[a.kind == KIND_I8 ? 0 : 1][a.gated];
+    kern = kPair[variant][a.gated];
   } else {
     // tokens of a tile: twice the even share, so that a moderate skew stays in one tile
     const int want = a.offsets ? (2 * avg < a.M ? 2 * avg : a.M) : a.M;
-    p.tok_max = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : 128;
+    p.tok_max = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 || seg ? 64 : 128;
     p.tok_round = 16;
+    p.band = 1 << 20;  // token blocks run fastest: neighbours share the weights
     p.num_w_blocks = (a.N + p.feats - 1) / p.feats;
     box = p.tok_max < 32 ? p.tok_max : 32;
     const int stage = W_BYTES + p.tok_max * BK;
@@ -996,7 +1220,7 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
     const long long clusters = tiles < ds->clusters[pick] ? tiles : ds->clusters[pick];
     cfg.gridDim = dim3((unsigned)(clusters * p.csize));
     cfg.blockDim = dim3(strm::THREADS);
-    kern = kStream[a.kind == KIND_I8 ? 0 : 1][a.gated];
+    kern = kStream[variant][a.gated];
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = p.csize;
     attr[1].val.clusterDim.y = 1;
@@ -1005,7 +1229,11 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
   }
   if (!make_map(&tmX, a.x, (uint64_t)a.K * es, (uint64_t)a.M, (uint64_t)a.ldx * es, box))
     return fail(QGEMM_ERR_CUDA, "cuTensorMapEncodeTiled failed for x");
-  return cuda_fail(cudaLaunchKernelEx(&cfg, kern, tmW, tmX, p), "linear launch");
+  CUtensorMap tmXs;
+  memset(&tmXs, 0, sizeof(tmXs));
+  if (use_pair && !make_map(&tmXs, a.x, (uint64_t)a.K * es, (uint64_t)a.M, (uint64_t)a.ldx * es, pair::BOX))
+    return fail(QGEMM_ERR_CUDA, "cuTensorMapEncodeTiled failed for x");
+  return cuda_fail(cudaLaunchKernelEx(&cfg, kern, tmW, tmG, tmX, tmXs, p), "linear launch");
 }
 
 }  // namespace qg

@@ -83,17 +83,21 @@ __device__ __forceinline__ int blocks_of(const Params& p, int cnt) {
   return (cnt + p.tok_max - 1) / p.tok_max;
 }
 
-// All threads: fills the table.  Offsets that are not 0 <= o[e] <= o[e+1] <= M name no rows.
+// One thread: the table of a dense layer, one group of M rows.
+__device__ __forceinline__ void dense_table(const Params& p, const Table& tb) {
+  tb.row0[0] = 0;
+  tb.cnt[0] = p.M;
+  tb.pref[0] = 0;
+  tb.pref[1] = blocks_of(p, p.M) * p.num_w_blocks;
+}
+
+// All threads: fills the experts' table.  Offsets that are not 0 <= o[e] <= o[e+1] <= M name no rows.
 __device__ __forceinline__ void fill_table(const Params& p, const Table& tb) {
   for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
-    int o0 = 0, o1 = p.M;
-    if (p.offsets) {
-      o0 = p.offsets[e];
-      o1 = p.offsets[e + 1];
-      if (o0 < 0 || o1 < o0 || o1 > p.M) {
-        if (p.err && blockIdx.x == 0) atomicCAS(p.err, 0, DEVERR_BAD_INDEX);
-        o0 = o1 = 0;
-      }
+    int o0 = p.offsets[e], o1 = p.offsets[e + 1];
+    if (o0 < 0 || o1 < o0 || o1 > p.M) {
+      if (p.err && blockIdx.x == 0) atomicCAS(p.err, 0, DEVERR_BAD_INDEX);
+      o0 = o1 = 0;
     }
     tb.row0[e] = o0;
     tb.cnt[e] = o1 - o0;
@@ -392,8 +396,14 @@ __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
   return v;
 }
 
-__device__ __forceinline__ void st_shared_u32(uint32_t addr, uint32_t v) {
-  asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+// Adds four accumulator words: int32, or fp32 rounding to nearest.
+template <int KIND>
+__device__ __forceinline__ void add_words(uint32_t (&a)[4], const uint4& v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    a[i] = KIND == KIND_I8 ? a[i] + w[i]
+                           : __float_as_uint(__fadd_rn(__uint_as_float(a[i]), __uint_as_float(w[i])));
 }
 
 // ---- the CTA-pair kernel -------------------------------------------------------------------
@@ -474,18 +484,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
     *abort_flag = 0;
     ptx::fence_mbar_init();
     ptx::grid_launch_dependents();
-    ptx::prefetch_tmap(&tmW);
+    ptx::prefetch_tmap(GATED ? &tmG : &tmW);
     ptx::prefetch_tmap(&tmX);
+    if (!p.offsets) dense_table(p, tb);
   }
   if (warp == 1) {
     ptx::tmem_alloc_pair(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
     ptx::tmem_relinquish_pair();
   }
-  ptx::grid_dependency_wait();  // the offsets, and everything below, may be the previous kernel's
-  fill_table(p, tb);
+  // everything up to here overlaps the previous kernel
   ptx::tc_fence_before();
   ptx::cluster_sync_all();
   ptx::tc_fence_after();
+  ptx::grid_dependency_wait();
+  if (p.offsets) fill_table(p, tb);
   const uint32_t tmem_base = *tmem_slot;
   Tile it_;
 
@@ -701,28 +713,32 @@ constexpr int THREADS = 192;   // producer, MMA issuer, four epilogue warps
 constexpr int SEG_TOK = 64;    // tokens of a tile at most with SEG
 }  // namespace strm
 
-template <int KIND, bool GATED, bool SEG>
+// SPLIT: a cluster of csize CTAs cuts K.  Every rank sends the sums of a token to the rank that
+// finishes it (st.async into that rank's receive buffer, counted in bytes on its barrier), which
+// adds them in rank order.  Otherwise a CTA finishes its own accumulator.
+template <int KIND, bool GATED, bool SEG, bool SPLIT>
 __global__ void __launch_bounds__(strm::THREADS, 1)
     linear_stream_kernel(const __grid_constant__ CUtensorMap tmW,
-                         const __grid_constant__ CUtensorMap, const __grid_constant__ CUtensorMap tmX,
+                         const __grid_constant__ CUtensorMap tmG,
+                         const __grid_constant__ CUtensorMap tmX,
                          const __grid_constant__ CUtensorMap, const Params p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_base = ptx::smem_u32(smem_raw);
   const uint32_t base = (raw_base + 1023u) & ~1023u;
   uint8_t* gbase = smem_raw + (base - raw_base);
-  const int S = p.stages, TOK = p.tok_max, C = p.csize;
+  const int S = p.stages, TOK = p.tok_max, C = SPLIT ? p.csize : 1;
   const int box = TOK < 32 ? TOK : 32;  // token rows of a TMA box
   const uint32_t stage_bytes = (uint32_t)(W_BYTES + TOK * BK);
-  // partial sums of this rank's tokens: [source rank][TOK / C tokens][128 features] words
+  // SPLIT: sums of this rank's tokens, [source rank][TOK / C tokens][128 weight rows] words
   const uint32_t recv = base + S * stage_bytes;
-  const uint32_t bar_base = recv + (uint32_t)TOK * WROWS * 4u;
+  const uint32_t bar_base = recv + (SPLIT ? (uint32_t)TOK * WROWS * 4u : 0u);
   uint8_t* gbar = gbase + (bar_base - base);
   auto full_bar = [&](int s) { return bar_base + 8u * s; };
   auto empty_bar = [&](int s) { return bar_base + 8u * (MAX_STAGES + s); };
   auto tfull_bar = [&](int a) { return bar_base + 8u * (2 * MAX_STAGES + a); };
   auto tempty_bar = [&](int a) { return bar_base + 8u * (2 * MAX_STAGES + 2 + a); };
   const uint32_t drain_bar = bar_base + 8u * (2 * MAX_STAGES + 4);
-  const uint32_t rfull_bar = bar_base + 8u * (2 * MAX_STAGES + 5);   // partial sums are in
+  const uint32_t rfull_bar = bar_base + 8u * (2 * MAX_STAGES + 5);   // all ranks' sums are in
   const uint32_t rempty_bar = bar_base + 8u * (2 * MAX_STAGES + 6);  // every rank has read its
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gbar + 8 * (2 * MAX_STAGES + 7));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gbar + 8 * (2 * MAX_STAGES + 7) + 4);
@@ -732,9 +748,9 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
   tb.pref = tb.cnt + p.E;
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int rank = C > 1 ? (int)ptx::cluster_ctarank() : 0;
+  const int rank = SPLIT ? (int)ptx::cluster_ctarank() : 0;
   const int cid = blockIdx.x / C, nclusters = gridDim.x / C;
-  const uint32_t tmem_cols = TOK < 16 ? 32u : 2u * TOK;  // TOK is 16, 32, 64 or 128
+  const uint32_t tmem_cols = 2u * TOK;  // 32, 64, 128 or 256
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
@@ -746,23 +762,25 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
       ptx::mbar_init(tempty_bar(a), 4);
     }
     ptx::mbar_init(drain_bar, 1);
-    ptx::mbar_init(rfull_bar, 4 * C);
+    ptx::mbar_init(rfull_bar, 1);
     ptx::mbar_init(rempty_bar, 4 * C);
     *abort_flag = 0;
     ptx::fence_mbar_init();
     ptx::grid_launch_dependents();
-    ptx::prefetch_tmap(&tmW);
+    ptx::prefetch_tmap(GATED ? &tmG : &tmW);
     ptx::prefetch_tmap(&tmX);
+    if (!p.offsets) dense_table(p, tb);
   }
   if (warp == 1) {
     ptx::tmem_alloc(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), tmem_cols);
     ptx::tmem_relinquish();
   }
-  ptx::grid_dependency_wait();
-  fill_table(p, tb);
+  // everything up to here overlaps the previous kernel
   ptx::tc_fence_before();
-  if (C > 1) ptx::cluster_sync_all(); else __syncthreads();
+  if (SPLIT) ptx::cluster_sync_all(); else __syncthreads();
   ptx::tc_fence_after();
+  ptx::grid_dependency_wait();
+  if (p.offsets) fill_table(p, tb);
   const uint32_t tmem_base = *tmem_slot;
   const int T = tb.pref[p.E];
   const int kb0 = (int)((long long)p.num_k_blocks * rank / C);
@@ -777,10 +795,9 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
       bool ok = true;
       for (int tile = cid; ok && tile < T; tile += nclusters) {
         const Tile t = tile_of(p, tb, tile, p.band);
-        if (t.n == 0) continue;
         const int boxes = (t.n + box - 1) / box;
         const uint32_t tx = W_BYTES + (uint32_t)(boxes * box * BK);
-        const int w0 = t.e * p.ep.nw + t.wb * p.feats;
+        const int f0 = t.wb * p.feats, w0 = t.e * p.ep.nw + f0;
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!ptx::mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.wait_ns)) {
             if (!*abort_flag) report_cluster(p.err, DEVERR_TIMEOUT_PRODUCER, abort_flag, C);
@@ -788,11 +805,22 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
             break;
           }
           const uint32_t sw = base + stage * stage_bytes, sx = sw + W_BYTES;
-          ptx::mbar_arrive_expect_tx(full_bar(stage), tx);
-          ptx::tma_load_2d(sw, &tmW, full_bar(stage), kb * BK, w0);
-          if (GATED) ptx::tma_load_2d(sw + W_BYTES / 2, &tmW, full_bar(stage), kb * BK, w0 + p.ep.N);
+          const uint32_t fb = full_bar(stage);
+          ptx::mbar_arrive_expect_tx(fb, tx);
+          if constexpr (GATED) {  // gate and up rows by turns of 16, as in the pair kernel
+            if (f0 + 64 <= p.ep.N / 16 * 16) {
+              ptx::tma_load_5d(sw, &tmG, fb, kb * BK, 0, 0, f0 / 16, t.e);
+            } else
+#pragma unroll
+              for (int b = 0; b < 4; ++b) {
+                ptx::tma_load_2d(sw + (2 * b) * 16 * BK, &tmW, fb, kb * BK, w0 + 16 * b);
+                ptx::tma_load_2d(sw + (2 * b + 1) * 16 * BK, &tmW, fb, kb * BK, w0 + p.ep.N + 16 * b);
+              }
+          } else {
+            ptx::tma_load_2d(sw, &tmW, fb, kb * BK, w0);
+          }
           for (int b = 0; b < boxes; ++b)
-            ptx::tma_load_2d(sx + b * box * BK, &tmX, full_bar(stage), kb * BK, t.t0 + b * box);
+            ptx::tma_load_2d(sx + b * box * BK, &tmX, fb, kb * BK, t.t0 + b * box);
           ++issued;
           if (++stage == S) { stage = 0; phase ^= 1u; }
         }
@@ -804,6 +832,8 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
         }
       }
     }
+    __syncwarp();
+    if (SPLIT) ptx::cluster_arrive();
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
     if (lane == 0) {
@@ -813,7 +843,6 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
       bool ok = true, issued_any = false;
       for (int tile = cid; ok && tile < T; tile += nclusters) {
         const Tile t = tile_of(p, tb, tile, p.band);
-        if (t.n == 0) continue;
         const int ncol = (t.n + 15) / 16 * 16;
         const uint32_t idesc = KIND == KIND_BF16 ? ptx::idesc_bf16(128, ncol)
                                                  : ptx::idesc_i8(128, ncol, false, false);
@@ -858,36 +887,59 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
           report_cluster(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag, C);
       }
     }
+    __syncwarp();
+    if (SPLIT) ptx::cluster_arrive();
   } else {
     // ---------------- epilogue ----------------
-    const int q = warp & 3;
+    const int q = warp & 3;     // TMEM lane quadrant
     const Epi& ep = p.ep;
-    const int slot = TOK / C;  // tokens of a rank's slice at most
+    const int slot = TOK / C;   // tokens of a rank's slice at most
+    const uint32_t tmem_q = tmem_base + ((uint32_t)(q * 32) << 16);
+    const uint32_t to0 = recv + (uint32_t)((rank * slot) * WROWS + q * 32 + lane) * 4u;
     int it = 0, tiles = 0;
-    bool ok = true;
+    bool ok = true, arrived = false;
     for (int tile = cid; ok && tile < T; tile += nclusters) {
       const Tile t = tile_of(p, tb, tile, p.band);
-      if (t.n == 0) continue;
+      const bool last_tile = tile + nclusters >= T;
+      const int f0 = t.wb * p.feats;
       const uint32_t xphase = (uint32_t)(tiles & 1);  // of the exchange barriers, one use a tile
       ++tiles;
       const int per = (t.n + C - 1) / C;              // rank r finishes tokens r * per ..
-      const int nf = t.wb * p.feats + 4 * (GATED ? lane % 16 : lane);
-      Feat<GATED> f;
-      load_feat<KIND, GATED>(ep, t.e, nf, f);
-      const uint32_t tmem_q = tmem_base + ((uint32_t)(q * 32) << 16);
-      const uint32_t to0 = recv + (uint32_t)((rank * slot) * WROWS + q * 32 + lane) * 4u;
+      const int mine = max(0, min(per, t.n - rank * per));
+      Feat<GATED> ff;
+      Lane<GATED> fl;
+      if (SPLIT) {
+        load_feat<KIND, GATED>(ep, t.e, f0 + 4 * (GATED ? lane % 16 : lane), ff);
+        if (threadIdx.x == 64)
+          ptx::mbar_arrive_expect_tx(rfull_bar, (uint32_t)(mine * C * WROWS) * 4u);
+      } else {
+        fl = lane_of<KIND, GATED>(ep, t.e, f0, q, lane);
+      }
       int dst = 0, tl = 0;
-      uint32_t to = ptx::map_to_rank(to0, 0);
-      // pushes 16 tokens' sums of this lane's weight row to the ranks that finish them
-      auto push = [&](int c, const uint32_t (&r)[16]) {
+      uint32_t to = 0, to_bar = 0;
+      if (SPLIT) {
+        to = ptx::map_to_rank(to0, 0);
+        to_bar = ptx::map_to_rank(rfull_bar, 0);
+      }
+      // 16 tokens' sums of this lane's weight row: finished here, or sent to the ranks that do
+      auto emit = [&](int c, const uint32_t (&r)[16]) {
+        if constexpr (!SPLIT) {
+          with_act(ep.act, [&](auto act) {
+            finish_chunk<KIND, GATED, decltype(act)::value>(ep, fl, t.t0 + c, t.n - c, lane, r, [] {});
+          });
+        } else {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          if (c + j < t.n) {
-            ptx::st_cluster_u32(to, r[j]);
-            to += WROWS * 4u;
-            if (++tl == per) {
-              tl = 0;
-              if (++dst < C) to = ptx::map_to_rank(to0, dst);
+          for (int j = 0; j < 16; ++j) {
+            if (c + j < t.n) {
+              ptx::st_async_u32(to, r[j], to_bar);
+              to += WROWS * 4u;
+              if (++tl == per) {
+                tl = 0;
+                if (++dst < C) {
+                  to = ptx::map_to_rank(to0, dst);
+                  to_bar = ptx::map_to_rank(rfull_bar, dst);
+                }
+              }
             }
           }
         }
@@ -897,7 +949,7 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
       for (int s0 = kb0; ok && s0 < kb1; s0 += seg, ++it) {
         const int a = it & 1;
         ok = ptx::mbar_wait(tfull_bar(a), (uint32_t)((it >> 1) & 1), abort_flag, p.wait_ns);
-        if (s0 + seg >= kb1)  // every rank has read the partial sums of the tile before
+        if (SPLIT && s0 + seg >= kb1)  // every rank has read the sums of the tile before
           ok = ok && ptx::mbar_wait_acquire_cluster(rempty_bar, xphase ^ 1u, abort_flag, p.wait_ns);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
@@ -907,7 +959,7 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
             uint32_t r[16];
             ptx::tmem_ld_32x32b_x16(tmem_q + (uint32_t)(a * TOK + c), r);
             ptx::tmem_wait_ld();
-            push(c, r);
+            emit(c, r);
           }
         } else {
 #pragma unroll
@@ -936,61 +988,58 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
             uint32_t r[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(run[i][j]);
-            push(16 * i, r);
+            emit(16 * i, r);
           }
       }
-      __syncwarp();
-      if (lane < C) ptx::mbar_arrive_release_cluster(ptx::map_to_rank(rfull_bar, lane));
-      ok = ptx::mbar_wait_acquire_cluster(rfull_bar, xphase, abort_flag, p.wait_ns);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) {
-        if (lane == 0 && !*abort_flag) report_cluster(p.err, DEVERR_TIMEOUT_EPILOGUE, abort_flag, C);
-        break;
-      }
-      const int mine = max(0, min(per, t.n - rank * per));
-      with_act(ep.act, [&](auto act) {
-        const int step = GATED ? 8 : 4;
-        for (int l = GATED ? (warp - 2) * 2 + lane / 16 : warp - 2; l < mine; l += step) {
-          const int row = t.t0 + rank * per + l;
-          if (f.n >= ep.N) continue;
-          float sx = 1.f, res[4];
-          if (KIND == KIND_I8) sx = __ldg(ep.sx + row);
-          load_residual(ep, row, f.n, res);
-          uint32_t g[4] = {0u, 0u, 0u, 0u}, u[4] = {0u, 0u, 0u, 0u};
-          for (int c = 0; c < C; ++c) {
-            const uint32_t at =
-                recv + (uint32_t)((c * slot + l) * WROWS + 4 * (GATED ? lane % 16 : lane)) * 4u;
-            const uint4 v = ld_shared_v4(at);
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              g[i] = KIND == KIND_I8 ? g[i] + w[i]
-                                     : __float_as_uint(__fadd_rn(__uint_as_float(g[i]), __uint_as_float(w[i])));
-            if (GATED) {
-              const uint4 v2 = ld_shared_v4(at + 64 * 4);
-              const uint32_t w2[4] = {v2.x, v2.y, v2.z, v2.w};
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                u[i] = KIND == KIND_I8 ? u[i] + w2[i]
-                                       : __float_as_uint(__fadd_rn(__uint_as_float(u[i]), __uint_as_float(w2[i])));
-            }
-          }
-          finish4<KIND, GATED, decltype(act)::value>(ep, f, row, sx, g, u, res);
+      if constexpr (SPLIT) {
+        ok = ptx::mbar_wait_acquire_cluster(rfull_bar, xphase, abort_flag, p.wait_ns);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) {
+          if (lane == 0 && !*abort_flag) report_cluster(p.err, DEVERR_TIMEOUT_EPILOGUE, abort_flag, C);
+          break;
         }
-      });
+        if (last_tile) {  // this warp has made its last access to another CTA
+          ptx::cluster_arrive();
+          arrived = true;
+        }
+        // words of this lane's four features in a token's 128: gated, gate rows then up rows
+        // by turns of 16
+        const int at0 = GATED ? (lane % 16) / 4 * 32 + (lane % 4) * 4 : 4 * lane;
+        with_act(ep.act, [&](auto act) {
+          for (int l = GATED ? (warp - 2) * 2 + lane / 16 : warp - 2; l < mine; l += GATED ? 8 : 4) {
+            const int row = t.t0 + rank * per + l;
+            if (ff.n >= ep.N) continue;
+            float sx = 1.f, res[4];
+            if (KIND == KIND_I8) sx = __ldg(ep.sx + row);
+            load_residual(ep, row, ff.n, res);
+            uint32_t g[4] = {0u, 0u, 0u, 0u}, u[4] = {0u, 0u, 0u, 0u};
+            for (int c = 0; c < C; ++c) {
+              const uint32_t at = recv + (uint32_t)((c * slot + l) * WROWS + at0) * 4u;
+              add_words<KIND>(g, ld_shared_v4(at));
+              if (GATED) add_words<KIND>(u, ld_shared_v4(at + 16 * 4));
+            }
+            finish4<KIND, GATED, decltype(act)::value>(ep, ff, row, sx, g, u, res);
+          }
+        });
+        __syncwarp();
+        if (!last_tile && lane < C)
+          ptx::mbar_arrive_release_cluster(ptx::map_to_rank(rempty_bar, lane));
+      }
+    }
+    if (SPLIT && !arrived) {
       __syncwarp();
-      if (lane < C) ptx::mbar_arrive_release_cluster(ptx::map_to_rank(rempty_bar, lane));
+      ptx::cluster_arrive();
     }
   }
 
   ptx::tc_fence_before();
   __syncthreads();
-  if (C > 1) ptx::cluster_sync_all();  // no CTA leaves while another writes or arrives in it
   ptx::tc_fence_after();
   if (warp == 1) {
     __syncwarp();
     ptx::tmem_dealloc(tmem_base, tmem_cols);
   }
+  if (SPLIT) ptx::cluster_wait();  // no CTA leaves while another may write or arrive in it
 }
 
 // ---- host side -----------------------------------------------------------------------------
@@ -1045,15 +1094,18 @@ static bool make_gated_map(CUtensorMap* m, const void* ptr, uint64_t width, int 
 
 using Kern = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const CUtensorMap,
                       const Params);
-// [int8, bf16, bf16 in segments][gated]
+// [int8, bf16, bf16 in segments][gated], the stream kernels also [K split]
 static const Kern kPair[3][2] = {
     {linear_pair_kernel<KIND_I8, false, false>, linear_pair_kernel<KIND_I8, true, false>},
     {linear_pair_kernel<KIND_BF16, false, false>, linear_pair_kernel<KIND_BF16, true, false>},
     {linear_pair_kernel<KIND_BF16, false, true>, linear_pair_kernel<KIND_BF16, true, true>}};
-static const Kern kStream[3][2] = {
-    {linear_stream_kernel<KIND_I8, false, false>, linear_stream_kernel<KIND_I8, true, false>},
-    {linear_stream_kernel<KIND_BF16, false, false>, linear_stream_kernel<KIND_BF16, true, false>},
-    {linear_stream_kernel<KIND_BF16, false, true>, linear_stream_kernel<KIND_BF16, true, true>}};
+static const Kern kStream[3][2][2] = {
+    {{linear_stream_kernel<KIND_I8, false, false, false>, linear_stream_kernel<KIND_I8, false, false, true>},
+     {linear_stream_kernel<KIND_I8, true, false, false>, linear_stream_kernel<KIND_I8, true, false, true>}},
+    {{linear_stream_kernel<KIND_BF16, false, false, false>, linear_stream_kernel<KIND_BF16, false, false, true>},
+     {linear_stream_kernel<KIND_BF16, true, false, false>, linear_stream_kernel<KIND_BF16, true, false, true>}},
+    {{linear_stream_kernel<KIND_BF16, false, true, false>, linear_stream_kernel<KIND_BF16, false, true, true>},
+     {linear_stream_kernel<KIND_BF16, true, true, false>, linear_stream_kernel<KIND_BF16, true, true, true>}}};
 
 // The tensor cores add each MMA's products to the fp32 accumulator by truncation, so a sum
 // over K shrinks by about 9e-10 of itself a value of K (measured: 2.1e-6 at K = 2048, 1.2e-5 at
@@ -1080,8 +1132,8 @@ static qgemm_status device_setup(qgemm_stream_s* s, const DeviceSetup** out) {
     for (int k = 0; k < 3; ++k)
       for (int g = 0; g < 2; ++g) {
         cudaError_t e = cudaFuncSetAttribute(kPair[k][g], cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
-        if (e == cudaSuccess)
-          e = cudaFuncSetAttribute(kStream[k][g], cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
+        for (int sp = 0; sp < 2 && e == cudaSuccess; ++sp)
+          e = cudaFuncSetAttribute(kStream[k][g][sp], cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
         if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(linear)");
       }
     for (int i = 0; i < 4; ++i) {
@@ -1098,7 +1150,7 @@ static qgemm_status device_setup(qgemm_stream_s* s, const DeviceSetup** out) {
       cfg.attrs = attr;
       cfg.numAttrs = 1;
       int n = 0;
-      const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kStream[0][0], &cfg);
+      const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kStream[0][0][1], &cfg);
       if (e != cudaSuccess) return cuda_fail(e, "cudaOccupancyMaxActiveClusters(linear)");
       d.clusters[i] = n;
     }
@@ -1154,14 +1206,14 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
   const int groups = a.E < a.M ? a.E : a.M;
   const int avg = (a.M + groups - 1) / groups;
   const bool use_pair = avg > 128;
-  // rows of a weight box: all of a CTA's, or one of its gate or up runs
-  const int w_rows = !a.gated ? WROWS : use_pair ? 16 : 64;
+  // rows of a weight box: all of a CTA's, or a run of gate or up rows
+  const int w_rows = a.gated ? 16 : WROWS;
   p.seg_kb = SEG_KB;
   const bool seg = a.kind == KIND_BF16 && a.out_dtype == QGEMM_F32 && p.num_k_blocks > SEG_KB;
   const int variant = a.kind == KIND_I8 ? 0 : seg ? 2 : 1;
   CUtensorMap tmW, tmG, tmX;
   memset(&tmG, 0, sizeof(tmG));
-  if (a.gated && use_pair && a.N >= 64 && !make_gated_map(&tmG, a.w, (uint64_t)a.K * es, a.N, a.E))
+  if (a.gated && a.N >= 64 && !make_gated_map(&tmG, a.w, (uint64_t)a.K * es, a.N, a.E))
     return fail(QGEMM_ERR_CUDA, "cuTensorMapEncodeTiled failed for the gated weights");
   if (!make_map(&tmW, a.w, (uint64_t)a.K * es, (uint64_t)a.E * p.ep.nw, (uint64_t)a.K * es, w_rows))
     return fail(QGEMM_ERR_CUDA, "cuTensorMapEncodeTiled failed for the weights");
@@ -1199,14 +1251,9 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
     p.band = 1 << 20;  // token blocks run fastest: neighbours share the weights
     p.num_w_blocks = (a.N + p.feats - 1) / p.feats;
     box = p.tok_max < 32 ? p.tok_max : 32;
-    const int stage = W_BYTES + p.tok_max * BK;
-    const int fixed = p.tok_max * WROWS * 4 + BAR_BYTES + table + 1024;
-    p.stages = (SMEM_MAX - fixed) / stage;
-    if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
-    cfg.dynamicSmemBytes = (size_t)fixed + (size_t)p.stages * stage;
     // Cut of K: rounds of tiles over the clusters that fit, times the k-blocks of a part,
     // plus a part's fixed cost (pipeline fill and exchange, about 3 k-blocks' time).
-    const long long tiles = (long long)p.num_w_blocks * ((a.M / p.tok_max) + groups);
+    const long long tiles = (long long)p.num_w_blocks * groups * ((avg + p.tok_max - 1) / p.tok_max);
     double best = 0;
     int pick = 0;
     for (int i = 0; i < 4; ++i) {
@@ -1217,10 +1264,18 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
       if (best == 0 || cost < best) { best = cost; pick = i; }
     }
     p.csize = 1 << pick;
-    const long long clusters = tiles < ds->clusters[pick] ? tiles : ds->clusters[pick];
+    const int stage = W_BYTES + p.tok_max * BK;
+    const int fixed = (p.csize > 1 ? p.tok_max * WROWS * 4 : 0) + BAR_BYTES + table + 1024;
+    p.stages = (SMEM_MAX - fixed) / stage;
+    if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
+    cfg.dynamicSmemBytes = (size_t)fixed + (size_t)p.stages * stage;
+    // as many clusters as fit (the counts of the experts are not known here: at least one
+    // tile each is not promised)
+    const long long most = (long long)p.num_w_blocks * (a.M / p.tok_max + groups);
+    const long long clusters = most < ds->clusters[pick] ? most : ds->clusters[pick];
     cfg.gridDim = dim3((unsigned)(clusters * p.csize));
     cfg.blockDim = dim3(strm::THREADS);
-    kern = kStream[variant][a.gated];
+    kern = kStream[variant][a.gated][p.csize > 1];
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = p.csize;
     attr[1].val.clusterDim.y = 1;

@@ -47,8 +47,8 @@ constexpr int WROWS = 128;      // weight rows of a CTA's tile
 constexpr int W_BYTES = WROWS * BK;          // 16 KB
 constexpr int CHUNK = 16;                    // accumulator columns (tokens) read at a time
 constexpr int SMEM_MAX = 232448;             // 227 KB
-constexpr int BAR_BYTES = 512;
-constexpr int MAX_STAGES = 12;
+constexpr int BAR_BYTES = 640;
+constexpr int MAX_STAGES = 32;
 
 struct Params {
   Epi ep;
@@ -59,7 +59,8 @@ struct Params {
   int tok_round;    // tokens of a tile are a multiple of this (MMA N)
   int num_w_blocks; // weight blocks of an expert
   int band;         // token blocks of a band of the schedule
-  int feats;        // features of a weight block of one CTA: 128, gated 64
+  int rows;         // weight rows of a CTA's tile: 128, in the stream kernel a multiple of 16
+  int feats;        // features of them: rows, gated rows / 2
   int stages;
   int seg_kb;       // k-blocks summed in TMEM before the sums move to registers (SEG)
   int csize;        // CTAs of a cluster (stream kernel)
@@ -169,6 +170,16 @@ __device__ __forceinline__ void report_cluster(int* err, int code, volatile int*
   for (int c = 0; c < csize; ++c) ptx::st_cluster_u32(ptx::map_to_rank(here, c), 1u);
 }
 
+// A whole warp waits; false (in every lane) when a lane's wait ran out, after reporting `code`.
+__device__ __forceinline__ bool warp_wait(const Params& p, uint32_t bar, uint32_t parity,
+                                          volatile int* abort_flag, int code, int csize) {
+  const bool ok = ptx::mbar_wait(bar, parity, abort_flag, p.wait_ns);
+  if (__all_sync(0xffffffffu, ok)) return true;
+  if (threadIdx.x % 32 == 0 && !*abort_flag) report_cluster(p.err, code, abort_flag, csize);
+  __syncwarp();
+  return false;
+}
+
 // ---- finishing four features of a token ---------------------------------------------------
 
 // Per-lane constants of a tile: this lane's four features (and, gated, their up rows).
@@ -253,8 +264,8 @@ __device__ __forceinline__ void finish4(const Epi& ep, const Feat<GATED>& f, int
 
 // ---- finishing a chunk of 16 tokens where the accumulator lies ------------------------------
 
-// A lane's weight row: its feature, scale and bias.  Gated: lanes 0-15 of a warp hold the gate
-// rows of 16 features, lanes 16-31 their up rows.
+// A lane's weight row: its feature (N or more: none), scale and bias.  Gated: a warp's lanes
+// hold 8 gate rows, the up rows of those 8 features, 8 gate rows and their up rows.
 template <bool GATED>
 struct Lane {
   int f;
@@ -262,10 +273,12 @@ struct Lane {
 };
 
 template <int KIND, bool GATED>
-__device__ __forceinline__ Lane<GATED> lane_of(const Epi& ep, int e, int f0, int q, int lane) {
+__device__ __forceinline__ Lane<GATED> lane_of(const Epi& ep, int e, int f0, int rows, int q,
+                                               int lane) {
   Lane<GATED> l;
-  l.f = f0 + (GATED ? q * 16 + lane % 16 : q * 32 + lane);
-  const size_t at = (size_t)e * ep.nw + l.f + (GATED && lane >= 16 ? ep.N : 0);
+  l.f = f0 + (GATED ? q * 16 + lane / 16 * 8 + lane % 8 : q * 32 + lane);
+  if (q * 32 + lane >= rows) l.f = ep.N + 2;  // its pair is past N too
+  const size_t at = (size_t)e * ep.nw + l.f + (GATED && (lane & 8) ? ep.N : 0);
   const bool in = l.f < ep.N;
   l.sw = KIND == KIND_I8 && in ? __ldg(ep.sw + at) : 0.f;
   l.b = ep.bias && in ? __ldg(ep.bias + at) : 0.f;
@@ -273,8 +286,8 @@ __device__ __forceinline__ Lane<GATED> lane_of(const Epi& ep, int e, int f0, int
 }
 
 // r: 16 accumulator columns (tokens row0 .. row0 + 15, of which `n` exist) of this lane's
-// weight row, valid after `ready`.  Gated, lanes l and l + 16 hold the gate and the up sums
-// of one feature: one shuffle a token pair gives lane l the even token and lane l + 16 the odd
+// weight row, valid after `ready`.  Gated, lanes l and l + 8 hold the gate and the up sums
+// of one feature: one shuffle a token pair gives lane l the even token and lane l + 8 the odd
 // one.  bf16 outputs are stored as feature pairs: one shuffle a token pair gives even lanes
 // both features of the first token and odd lanes those of the second, so that a warp's store
 // covers whole 32-byte sectors of two (gated: four) token rows.  Stores go straight to memory:
@@ -285,7 +298,7 @@ template <int KIND, bool GATED, int ACT, bool FULL, typename Ready>
 __device__ __forceinline__ void finish_chunk_t(const Epi& ep, const Lane<GATED>& l, int row0, int n,
                                                int lane, const uint32_t (&r)[16], Ready&& ready) {
   constexpr int NV = GATED ? 8 : 16;       // values a lane finishes
-  const int hi = GATED ? lane / 16 : 0;    // value i is token (GATED ? 2 i + hi : i)
+  const int hi = GATED ? lane / 8 % 2 : 0; // value i is token (GATED ? 2 i + hi : i)
   const int fe = l.f & ~1;                 // packed: features fe, fe + 1
   const int odd = l.f & 1;
   const bool packed = !ep.out_f32 && ep.vec2;
@@ -328,7 +341,7 @@ __device__ __forceinline__ void finish_chunk_t(const Epi& ep, const Lane<GATED>&
   if constexpr (GATED) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float other = __shfl_xor_sync(0xffffffffu, hi ? v[2 * i] : v[2 * i + 1], 16);
+      const float other = __shfl_xor_sync(0xffffffffu, hi ? v[2 * i] : v[2 * i + 1], 8);
       const float gate = hi ? other : v[2 * i], up = hi ? v[2 * i + 1] : other;
       v[i] = __fmul_rn(activate(ACT, gate), up);
     }
@@ -368,8 +381,7 @@ __device__ __forceinline__ void finish_chunk_t(const Epi& ep, const Lane<GATED>&
 template <int KIND, bool GATED, int ACT, typename Ready>
 __device__ __forceinline__ void finish_chunk(const Epi& ep, const Lane<GATED>& l, int row0, int n,
                                              int lane, const uint32_t (&r)[16], Ready&& ready) {
-  const int last = l.f - (GATED ? lane % 16 - 15 : lane - 31);  // the warp's last feature
-  if (n >= 16 && last < ep.N)
+  if (n >= 16 && __all_sync(0xffffffffu, l.f < ep.N))
     finish_chunk_t<KIND, GATED, ACT, true>(ep, l, row0, n, lane, r, ready);
   else
     finish_chunk_t<KIND, GATED, ACT, false>(ep, l, row0, n, lane, r, ready);
@@ -394,6 +406,10 @@ __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
                : "r"(addr)
                : "memory");
   return v;
+}
+
+__device__ __forceinline__ void st_shared_u32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
 // Adds four accumulator words: int32, or fp32 rounding to nearest.
@@ -503,43 +519,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
 
   if (warp == 0) {
     // ---------------- TMA producer (both CTAs) ----------------
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      long long issued = 0;
-      bool ok = true;
-      for (int item = 0; ok && pair_item(p, tb, pid, npairs, item, it_); ++item) {
-        if (it_.n == 0) continue;
-        const int half = (it_.n + p.tok_round - 1) / p.tok_round * p.tok_round / 2;
-        const int boxes = (half + pair::BOX - 1) / pair::BOX;  // 1 to 4
-        const uint32_t tx = 2u * (W_BYTES + (uint32_t)boxes * pair::BOX * BK);
-        const int x0 = it_.t0 + (int)rank * half;
-        // this CTA's weight rows: 128 of the block's 256, or 64 gate and 64 up rows
-        const int f0 = (it_.wb * 2 + (int)rank) * p.feats;
-        const int w0 = it_.e * p.ep.nw + f0;
-        for (int kb = 0; kb < p.num_k_blocks; ++kb) {
-          if (!ptx::mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.wait_ns)) {
-            if (!*abort_flag) report_cluster(p.err, DEVERR_TIMEOUT_PRODUCER, abort_flag, 2);
-            ok = false;
-            break;
-          }
+    int stage = 0;
+    uint32_t phase = 0;
+    long long issued = 0;
+    bool ok = true;
+    for (int item = 0; ok && pair_item(p, tb, pid, npairs, item, it_); ++item) {
+      if (it_.n == 0) continue;
+      const int half = (it_.n + p.tok_round - 1) / p.tok_round * p.tok_round / 2;
+      const int boxes = (half + pair::BOX - 1) / pair::BOX;  // 1 to 4
+      const uint32_t tx = 2u * (W_BYTES + (uint32_t)boxes * pair::BOX * BK);
+      const int x0 = it_.t0 + (int)rank * half;
+      // this CTA's weight rows: 128 of the block's 256, or 64 gate and 64 up rows
+      const int f0 = (it_.wb * 2 + (int)rank) * p.feats;
+      const int w0 = it_.e * p.ep.nw + f0;
+      for (int kb = 0; kb < p.num_k_blocks; ++kb) {
+        if (!warp_wait(p, empty_bar(stage), phase ^ 1u, abort_flag, DEVERR_TIMEOUT_PRODUCER, 2)) {
+          ok = false;
+          break;
+        }
+        if (ptx::elect_one()) {
           const uint32_t sw = base + stage * pair::STAGE_BYTES, sx = sw + W_BYTES;
           const uint32_t fb = ptx::map_to_rank(full_bar(stage), 0);
           if (rank == 0) ptx::mbar_arrive_expect_tx(full_bar(stage), tx);
           if constexpr (GATED) {
-            // 16 gate rows, the 16 up rows of the same features, and so on: both halves of
-            // a feature's product land in one warp's TMEM lanes.  One copy through the 5-D
-            // map (k, row of 16, gate / up, block of 16 features, expert) where all 64
-            // features lie in whole blocks, else eight (the last features of an N that is
-            // not a multiple of 16; eight copies for every tile made the layer 25 % slower)
-            if (f0 + 64 <= p.ep.N / 16 * 16) {
-              ptx::tma_load_5d_pair(sw, &tmG, fb, kb * BK, 0, 0, f0 / 16, it_.e);
-            } else
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-              ptx::tma_load_2d_pair(sw + (2 * b) * 16 * BK, &tmW, fb, kb * BK, w0 + 16 * b);
-              ptx::tma_load_2d_pair(sw + (2 * b + 1) * 16 * BK, &tmW, fb, kb * BK,
-                                    w0 + p.ep.N + 16 * b);
+            // 8 gate rows, the 8 up rows of the same features, and so on: both halves of a
+            // feature's product land in one warp's TMEM lanes.  One copy through the 5-D map
+            // (k, row of 8, gate / up, block of 8 features, expert) where all 64 features lie
+            // in whole blocks, else one copy for every 8 rows (the last features of an N that
+            // is not a multiple of 8; eight copies for every tile made the layer 25 % slower)
+            if (f0 + 64 <= p.ep.N / 8 * 8) {
+              ptx::tma_load_5d_pair(sw, &tmG, fb, kb * BK, 0, 0, f0 / 8, it_.e);
+            } else {
+              for (int b = 0; b < 8; ++b) {
+                ptx::tma_load_2d_pair(sw + (2 * b) * 8 * BK, &tmW, fb, kb * BK, w0 + 8 * b);
+                ptx::tma_load_2d_pair(sw + (2 * b + 1) * 8 * BK, &tmW, fb, kb * BK, w0 + p.ep.N + 8 * b);
+              }
             }
           } else {
             ptx::tma_load_2d_pair(sw, &tmW, fb, kb * BK, w0);
@@ -549,23 +563,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
           else
             for (int b = 0; b < boxes; ++b)
               ptx::tma_load_2d_pair(sx + b * pair::BOX * BK, &tmXs, fb, kb * BK, x0 + b * pair::BOX);
-          ++issued;
-          if (++stage == S) { stage = 0; phase ^= 1u; }
         }
+        __syncwarp();
+        ++issued;
+        if (++stage == S) { stage = 0; phase ^= 1u; }
       }
-      // Drain: the even CTA's full barriers count both CTAs' copies.
-      if (rank == 0) {
-        for (long long f = (issued > S ? issued - S : 0); f < issued; ++f) {
-          if (!ptx::mbar_wait(full_bar((int)(f % S)), (uint32_t)((f / S) & 1), nullptr, p.wait_ns)) {
-            report_cluster(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag, 2);
-            break;
-          }
+    }
+    // Drain: the even CTA's full barriers count both CTAs' copies.
+    if (rank == 0 && lane == 0) {
+      for (long long f = (issued > S ? issued - S : 0); f < issued; ++f) {
+        if (!ptx::mbar_wait(full_bar((int)(f % S)), (uint32_t)((f / S) & 1), nullptr, p.wait_ns)) {
+          report_cluster(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag, 2);
+          break;
         }
       }
     }
+    __syncwarp();
   } else if (warp == 1) {
     // ---------------- MMA issuer (even CTA) ----------------
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       int stage = 0;
       uint32_t phase = 0;
       int it = 0;
@@ -578,8 +594,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
         const int seg = SEG ? p.seg_kb : p.num_k_blocks;
         for (int kb0 = 0; ok && kb0 < p.num_k_blocks; kb0 += seg) {
           const int a = it & 1;
-          if (!ptx::mbar_wait(tempty_bar(a), (uint32_t)((it >> 1) & 1) ^ 1u, abort_flag, p.wait_ns)) {
-            if (!*abort_flag) report_cluster(p.err, DEVERR_TIMEOUT_MMA, abort_flag, 2);
+          if (!warp_wait(p, tempty_bar(a), (uint32_t)((it >> 1) & 1) ^ 1u, abort_flag,
+                         DEVERR_TIMEOUT_MMA, 2)) {
             ok = false;
             break;
           }
@@ -588,33 +604,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
           const uint32_t d_tmem = tmem_base + (uint32_t)(a * 256);
           const int kb1 = min(kb0 + seg, p.num_k_blocks);
           for (int kb = kb0; kb < kb1; ++kb) {
-            if (!ptx::mbar_wait(full_bar(stage), phase, abort_flag, p.wait_ns)) {
-              if (!*abort_flag) report_cluster(p.err, DEVERR_TIMEOUT_MMA, abort_flag, 2);
+            if (!warp_wait(p, full_bar(stage), phase, abort_flag, DEVERR_TIMEOUT_MMA, 2)) {
               ok = false;
               break;
             }
             ptx::tc_fence_after();
-            const uint32_t sw = base + stage * pair::STAGE_BYTES, sx = sw + W_BYTES;
-            const uint32_t empty = empty_bar(stage);
-            if (++stage == S) { stage = 0; phase ^= 1u; }
+            if (ptx::elect_one()) {
+              const uint32_t sw = base + stage * pair::STAGE_BYTES;
+              const uint64_t adesc = ptx::smem_desc_sw128(sw, 16, 1024);
+              const uint64_t bdesc = ptx::smem_desc_sw128(sw + W_BYTES, 16, 1024);
 #pragma unroll
-            for (int kk = 0; kk < BK / UMMA_K; ++kk) {
-              const uint64_t adesc = ptx::smem_desc_sw128(sw + kk * UMMA_K, 16, 1024);
-              const uint64_t bdesc = ptx::smem_desc_sw128(sx + kk * UMMA_K, 16, 1024);
-              const uint32_t accum = (kb != kb0 || kk != 0) ? 1u : 0u;
-              if constexpr (KIND == KIND_BF16) ptx::umma_bf16_pair(d_tmem, adesc, bdesc, idesc, accum);
-              else ptx::umma_i8_pair(d_tmem, adesc, bdesc, idesc, accum);
+              for (int kk = 0; kk < BK / UMMA_K; ++kk) {  // 32 bytes further along the swizzled rows
+                const uint32_t accum = (kb != kb0 || kk != 0) ? 1u : 0u;
+                if constexpr (KIND == KIND_BF16)
+                  ptx::umma_bf16_pair(d_tmem, adesc + kk * (UMMA_K / 16), bdesc + kk * (UMMA_K / 16), idesc, accum);
+                else
+                  ptx::umma_i8_pair(d_tmem, adesc + kk * (UMMA_K / 16), bdesc + kk * (UMMA_K / 16), idesc, accum);
+              }
+              ptx::umma_commit_pair(empty_bar(stage), 0x3);
+              if (kb + 1 == kb1) ptx::umma_commit_pair(tfull_bar(a), 0x3);
             }
-            ptx::umma_commit_pair(empty, 0x3);
+            __syncwarp();
             issued_any = true;
+            if (++stage == S) { stage = 0; phase ^= 1u; }
           }
-          if (ok) ptx::umma_commit_pair(tfull_bar(a), 0x3);
         }
       }
       if (!ok && issued_any) {
-        ptx::umma_commit_pair(drain_bar, 0x1);
-        if (!ptx::mbar_wait(drain_bar, 0, nullptr, p.wait_ns))
+        if (ptx::elect_one()) ptx::umma_commit_pair(drain_bar, 0x1);
+        __syncwarp();
+        if (lane == 0 && !ptx::mbar_wait(drain_bar, 0, nullptr, p.wait_ns))
           report_cluster(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag, 2);
+        __syncwarp();
       }
     }
   } else {
@@ -628,7 +649,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
     for (int item = 0; pair_item(p, tb, pid, npairs, item, it_); ++item) {
       if (it_.n == 0) continue;
       const Lane<GATED> f =
-          lane_of<KIND, GATED>(p.ep, it_.e, (it_.wb * 2 + (int)rank) * p.feats, q, lane);
+          lane_of<KIND, GATED>(p.ep, it_.e, (it_.wb * 2 + (int)rank) * p.feats, WROWS, q, lane);
       const int chunks = (it_.n + CHUNK - 1) / CHUNK;
       // Waits for accumulator it & 1; a warp whose wait ran out stores nothing.
       auto acc_ready = [&]() {
@@ -711,11 +732,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
 namespace strm {  // tiles of 16, 32, 64 or 128 tokens at most (Params::tok_max)
 constexpr int THREADS = 192;   // producer, MMA issuer, four epilogue warps
 constexpr int SEG_TOK = 64;    // tokens of a tile at most with SEG
+constexpr int XTOK = 64;       // tokens of an exchange at most (SPLIT)
 }  // namespace strm
 
-// SPLIT: a cluster of csize CTAs cuts K.  Every rank sends the sums of a token to the rank that
-// finishes it (st.async into that rank's receive buffer, counted in bytes on its barrier), which
-// adds them in rank order.  Otherwise a CTA finishes its own accumulator.
+// SPLIT: a cluster of csize CTAs cuts K.  The sums of a token go to the rank that finishes it,
+// which adds them in rank order: each warp lays its 32 weight rows' sums out in shared memory
+// ([token][32]) and sends every rank its run of tokens as one bulk copy, counted in bytes on the
+// receiver's barrier (word by word with st.async, 33 tokens took 2700 cycles a tile and 128
+// took 8500; DSMEM moves wide runs far better).  Otherwise a CTA finishes its own accumulator.
 template <int KIND, bool GATED, bool SEG, bool SPLIT>
 __global__ void __launch_bounds__(strm::THREADS, 1)
     linear_stream_kernel(const __grid_constant__ CUtensorMap tmW,
@@ -728,10 +752,14 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
   uint8_t* gbase = smem_raw + (base - raw_base);
   const int S = p.stages, TOK = p.tok_max, C = SPLIT ? p.csize : 1;
   const int box = TOK < 32 ? TOK : 32;  // token rows of a TMA box
-  const uint32_t stage_bytes = (uint32_t)(W_BYTES + TOK * BK);
-  // SPLIT: sums of this rank's tokens, [source rank][TOK / C tokens][128 weight rows] words
-  const uint32_t recv = base + S * stage_bytes;
-  const uint32_t bar_base = recv + (SPLIT ? (uint32_t)TOK * WROWS * 4u : 0u);
+  const uint32_t w_bytes = (uint32_t)(p.rows * BK);
+  const uint32_t stage_bytes = w_bytes + (uint32_t)(TOK * BK);
+  // SPLIT: the sums that this rank sends, [warp][token][32 weight rows] words, and those of its
+  // own tokens, [source rank][warp][XT / C tokens][32]
+  const int XT = min(TOK, strm::XTOK);
+  const uint32_t send = base + S * stage_bytes;
+  const uint32_t recv = send + (SPLIT ? (uint32_t)XT * WROWS * 4u : 0u);
+  const uint32_t bar_base = recv + (SPLIT ? (uint32_t)XT * WROWS * 4u : 0u);
   uint8_t* gbar = gbase + (bar_base - base);
   auto full_bar = [&](int s) { return bar_base + 8u * s; };
   auto empty_bar = [&](int s) { return bar_base + 8u * (MAX_STAGES + s); };
@@ -788,104 +816,110 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
 
   if (warp == 0) {
     // ---------------- TMA producer ----------------
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      long long issued = 0;
-      bool ok = true;
-      for (int tile = cid; ok && tile < T; tile += nclusters) {
-        const Tile t = tile_of(p, tb, tile, p.band);
-        const int boxes = (t.n + box - 1) / box;
-        const uint32_t tx = W_BYTES + (uint32_t)(boxes * box * BK);
-        const int f0 = t.wb * p.feats, w0 = t.e * p.ep.nw + f0;
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (!ptx::mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.wait_ns)) {
-            if (!*abort_flag) report_cluster(p.err, DEVERR_TIMEOUT_PRODUCER, abort_flag, C);
-            ok = false;
-            break;
-          }
-          const uint32_t sw = base + stage * stage_bytes, sx = sw + W_BYTES;
+    int stage = 0;
+    uint32_t phase = 0;
+    long long issued = 0;
+    bool ok = true;
+    for (int tile = cid; ok && tile < T; tile += nclusters) {
+      const Tile t = tile_of(p, tb, tile, p.band);
+      const int boxes = (t.n + box - 1) / box;
+      const uint32_t tx = w_bytes + (uint32_t)(boxes * box * BK);
+      const int f0 = t.wb * p.feats, w0 = t.e * p.ep.nw + f0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!warp_wait(p, empty_bar(stage), phase ^ 1u, abort_flag, DEVERR_TIMEOUT_PRODUCER, C)) {
+          ok = false;
+          break;
+        }
+        if (ptx::elect_one()) {
+          const uint32_t sw = base + stage * stage_bytes, sx = sw + w_bytes;
           const uint32_t fb = full_bar(stage);
           ptx::mbar_arrive_expect_tx(fb, tx);
-          if constexpr (GATED) {  // gate and up rows by turns of 16, as in the pair kernel
-            if (f0 + 64 <= p.ep.N / 16 * 16) {
-              ptx::tma_load_5d(sw, &tmG, fb, kb * BK, 0, 0, f0 / 16, t.e);
-            } else
-#pragma unroll
-              for (int b = 0; b < 4; ++b) {
-                ptx::tma_load_2d(sw + (2 * b) * 16 * BK, &tmW, fb, kb * BK, w0 + 16 * b);
-                ptx::tma_load_2d(sw + (2 * b + 1) * 16 * BK, &tmW, fb, kb * BK, w0 + p.ep.N + 16 * b);
+          if constexpr (GATED) {  // gate and up rows by turns of 8, as in the pair kernel
+            if (f0 + p.feats <= p.ep.N / 8 * 8) {
+              ptx::tma_load_5d(sw, &tmG, fb, kb * BK, 0, 0, f0 / 8, t.e);
+            } else {
+              for (int b = 0; b < p.feats / 8; ++b) {
+                ptx::tma_load_2d(sw + (2 * b) * 8 * BK, &tmW, fb, kb * BK, w0 + 8 * b);
+                ptx::tma_load_2d(sw + (2 * b + 1) * 8 * BK, &tmW, fb, kb * BK, w0 + p.ep.N + 8 * b);
               }
+            }
           } else {
             ptx::tma_load_2d(sw, &tmW, fb, kb * BK, w0);
           }
           for (int b = 0; b < boxes; ++b)
             ptx::tma_load_2d(sx + b * box * BK, &tmX, fb, kb * BK, t.t0 + b * box);
-          ++issued;
-          if (++stage == S) { stage = 0; phase ^= 1u; }
         }
+        __syncwarp();
+        ++issued;
+        if (++stage == S) { stage = 0; phase ^= 1u; }
       }
+    }
+    if (lane == 0)
       for (long long f = (issued > S ? issued - S : 0); f < issued; ++f) {
         if (!ptx::mbar_wait(full_bar((int)(f % S)), (uint32_t)((f / S) & 1), nullptr, p.wait_ns)) {
           report_cluster(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag, C);
           break;
         }
       }
-    }
     __syncwarp();
     if (SPLIT) ptx::cluster_arrive();
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      int it = 0;
-      bool ok = true, issued_any = false;
-      for (int tile = cid; ok && tile < T; tile += nclusters) {
-        const Tile t = tile_of(p, tb, tile, p.band);
-        const int ncol = (t.n + 15) / 16 * 16;
-        const uint32_t idesc = KIND == KIND_BF16 ? ptx::idesc_bf16(128, ncol)
-                                                 : ptx::idesc_i8(128, ncol, false, false);
-        const int seg = SEG ? p.seg_kb : p.num_k_blocks;
-        for (int s0 = kb0; ok && s0 < kb1; s0 += seg) {
-          const int a = it & 1;
-          if (!ptx::mbar_wait(tempty_bar(a), (uint32_t)((it >> 1) & 1) ^ 1u, abort_flag, p.wait_ns)) {
-            if (!*abort_flag) report_cluster(p.err, DEVERR_TIMEOUT_MMA, abort_flag, C);
+    int stage = 0;
+    uint32_t phase = 0;
+    int it = 0;
+    bool ok = true, issued_any = false;
+    for (int tile = cid; ok && tile < T; tile += nclusters) {
+      const Tile t = tile_of(p, tb, tile, p.band);
+      const int ncol = (t.n + 15) / 16 * 16;
+      const uint32_t idesc = KIND == KIND_BF16 ? ptx::idesc_bf16(128, ncol)
+                                               : ptx::idesc_i8(128, ncol, false, false);
+      const int seg = SEG ? p.seg_kb : p.num_k_blocks;
+      for (int s0 = kb0; ok && s0 < kb1; s0 += seg) {
+        const int a = it & 1;
+        if (!warp_wait(p, tempty_bar(a), (uint32_t)((it >> 1) & 1) ^ 1u, abort_flag,
+                       DEVERR_TIMEOUT_MMA, C)) {
+          ok = false;
+          break;
+        }
+        ++it;
+        ptx::tc_fence_after();
+        const uint32_t d_tmem = tmem_base + (uint32_t)(a * TOK);
+        const int s1 = min(s0 + seg, kb1);
+        for (int kb = s0; kb < s1; ++kb) {
+          if (!warp_wait(p, full_bar(stage), phase, abort_flag, DEVERR_TIMEOUT_MMA, C)) {
             ok = false;
             break;
           }
-          ++it;
           ptx::tc_fence_after();
-          const uint32_t d_tmem = tmem_base + (uint32_t)(a * TOK);
-          const int s1 = min(s0 + seg, kb1);
-          for (int kb = s0; kb < s1; ++kb) {
-            if (!ptx::mbar_wait(full_bar(stage), phase, abort_flag, p.wait_ns)) {
-              if (!*abort_flag) report_cluster(p.err, DEVERR_TIMEOUT_MMA, abort_flag, C);
-              ok = false;
-              break;
-            }
-            ptx::tc_fence_after();
-            const uint32_t sw = base + stage * stage_bytes, sx = sw + W_BYTES;
+          if (ptx::elect_one()) {
+            // the MMA reads 128 weight rows: past p.rows they are whatever the ring holds, and
+            // only lanes that nothing reads see them
+            const uint32_t sw = base + stage * stage_bytes;
+            const uint64_t adesc = ptx::smem_desc_sw128(sw, 16, 1024);
+            const uint64_t bdesc = ptx::smem_desc_sw128(sw + w_bytes, 16, 1024);
 #pragma unroll
             for (int kk = 0; kk < BK / UMMA_K; ++kk) {
-              const uint64_t adesc = ptx::smem_desc_sw128(sw + kk * UMMA_K, 16, 1024);
-              const uint64_t bdesc = ptx::smem_desc_sw128(sx + kk * UMMA_K, 16, 1024);
               const uint32_t accum = (kb != s0 || kk != 0) ? 1u : 0u;
-              if constexpr (KIND == KIND_BF16) ptx::umma_bf16(d_tmem, adesc, bdesc, idesc, accum);
-              else ptx::umma_i8(d_tmem, adesc, bdesc, idesc, accum);
+              if constexpr (KIND == KIND_BF16)
+                ptx::umma_bf16(d_tmem, adesc + kk * (UMMA_K / 16), bdesc + kk * (UMMA_K / 16), idesc, accum);
+              else
+                ptx::umma_i8(d_tmem, adesc + kk * (UMMA_K / 16), bdesc + kk * (UMMA_K / 16), idesc, accum);
             }
             ptx::umma_commit(empty_bar(stage));
-            issued_any = true;
-            if (++stage == S) { stage = 0; phase ^= 1u; }
+            if (kb + 1 == s1) ptx::umma_commit(tfull_bar(a));
           }
-          if (ok) ptx::umma_commit(tfull_bar(a));
+          __syncwarp();
+          issued_any = true;
+          if (++stage == S) { stage = 0; phase ^= 1u; }
         }
       }
-      if (!ok && issued_any) {
-        ptx::umma_commit(drain_bar);
-        if (!ptx::mbar_wait(drain_bar, 0, nullptr, p.wait_ns))
-          report_cluster(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag, C);
-      }
+    }
+    if (!ok && issued_any) {
+      if (ptx::elect_one()) ptx::umma_commit(drain_bar);
+      __syncwarp();
+      if (lane == 0 && !ptx::mbar_wait(drain_bar, 0, nullptr, p.wait_ns))
+        report_cluster(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag, C);
     }
     __syncwarp();
     if (SPLIT) ptx::cluster_arrive();
@@ -893,55 +927,100 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
     // ---------------- epilogue ----------------
     const int q = warp & 3;     // TMEM lane quadrant
     const Epi& ep = p.ep;
-    const int slot = TOK / C;   // tokens of a rank's slice at most
+    const int w4 = warp - 2;
+    const int slot = XT / C;    // tokens of a rank's slice at most
     const uint32_t tmem_q = tmem_base + ((uint32_t)(q * 32) << 16);
-    const uint32_t to0 = recv + (uint32_t)((rank * slot) * WROWS + q * 32 + lane) * 4u;
-    int it = 0, tiles = 0;
+    const uint32_t send_q = send + (uint32_t)(q * XT) * 128u;  // this warp's part
+    int it = 0, xc = 0;         // accumulators read, exchanges made
     bool ok = true, arrived = false;
     for (int tile = cid; ok && tile < T; tile += nclusters) {
       const Tile t = tile_of(p, tb, tile, p.band);
       const bool last_tile = tile + nclusters >= T;
       const int f0 = t.wb * p.feats;
-      const uint32_t xphase = (uint32_t)(tiles & 1);  // of the exchange barriers, one use a tile
-      ++tiles;
-      const int per = (t.n + C - 1) / C;              // rank r finishes tokens r * per ..
-      const int mine = max(0, min(per, t.n - rank * per));
       Feat<GATED> ff;
       Lane<GATED> fl;
       if (SPLIT) {
-        load_feat<KIND, GATED>(ep, t.e, f0 + 4 * (GATED ? lane % 16 : lane), ff);
+        const int f4 = 4 * (GATED ? lane % 16 : lane);
+        load_feat<KIND, GATED>(ep, t.e, f4 < p.feats ? f0 + f4 : ep.N, ff);
+      }
+      else fl = lane_of<KIND, GATED>(ep, t.e, f0, p.rows, q, lane);
+      // One exchange: tokens x0 .. x0 + xn of the tile, whose sums this warp has laid out.
+      auto exchange = [&](int x0, int xn) {
+        const uint32_t phase = (uint32_t)(xc & 1);
+        ++xc;
+        const int per = (xn + C - 1) / C;          // rank r finishes tokens r * per ..
+        const int mine = max(0, min(per, xn - rank * per));
+        const int row0 = t.t0 + x0 + rank * per;
+        // the scales of this rank's tokens (32 at most), while the copies are under way
+        float sxl = 1.f;
+        if (KIND == KIND_I8 && lane < mine) sxl = __ldg(ep.sx + row0 + lane);
         if (threadIdx.x == 64)
           ptx::mbar_arrive_expect_tx(rfull_bar, (uint32_t)(mine * C * WROWS) * 4u);
-      } else {
-        fl = lane_of<KIND, GATED>(ep, t.e, f0, q, lane);
-      }
-      int dst = 0, tl = 0;
-      uint32_t to = 0, to_bar = 0;
-      if (SPLIT) {
-        to = ptx::map_to_rank(to0, 0);
-        to_bar = ptx::map_to_rank(rfull_bar, 0);
-      }
-      // 16 tokens' sums of this lane's weight row: finished here, or sent to the ranks that do
+        ptx::fence_proxy_async_smem();             // the layout -> visible to the bulk copies
+        __syncwarp();
+        if (lane < C) {
+          const int theirs = max(0, min(per, xn - lane * per));
+          if (theirs > 0)
+            ptx::bulk_copy_cluster(ptx::map_to_rank(recv + (uint32_t)((rank * 4 + q) * slot) * 128u, lane),
+                                   send_q + (uint32_t)(lane * per) * 128u, (uint32_t)theirs * 128u,
+                                   ptx::map_to_rank(rfull_bar, lane));
+        }
+        ok = ptx::mbar_wait_acquire_cluster(rfull_bar, phase, abort_flag, p.wait_ns);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return;
+        const bool last = last_tile && x0 + xn >= t.n;
+        if (last) {  // this warp has made its last access to another CTA
+          ptx::cluster_arrive();
+          arrived = true;
+        }
+        // this lane's four features in a source's [warp][slot][32] words: gated, gate rows and
+        // up rows by turns of 8
+        const int fq = GATED ? (lane % 16) / 4 : lane / 8;
+        const int fw = GATED ? lane / 2 % 2 * 16 + lane % 2 * 4 : (lane % 8) * 4;
+        with_act(ep.act, [&](auto act) {
+          const int step = GATED ? 8 : 4;
+          for (int l0 = GATED ? w4 * 2 : w4; l0 < mine; l0 += step) {  // warp-uniform
+            const int l = l0 + (GATED ? lane / 16 : 0);
+            const float sx = __shfl_sync(0xffffffffu, sxl, l & 31);
+            if (l >= mine || ff.n >= ep.N) continue;
+            float res[4];
+            load_residual(ep, row0 + l, ff.n, res);
+            uint32_t g[4] = {0u, 0u, 0u, 0u}, u[4] = {0u, 0u, 0u, 0u};
+            for (int c = 0; c < C; ++c) {
+              const uint32_t at = recv + (uint32_t)(((c * 4 + fq) * slot + l) * 32 + fw) * 4u;
+              add_words<KIND>(g, ld_shared_v4(at));
+              if (GATED) add_words<KIND>(u, ld_shared_v4(at + 8 * 4));
+            }
+            finish4<KIND, GATED, decltype(act)::value>(ep, ff, row0 + l, sx, g, u, res);
+          }
+        });
+        __syncwarp();
+        // The loads above have returned (their values went into the outputs), so the arrival
+        // needs no release: a cluster-scope one waited for the output stores, 2000 cycles a
+        // tile.
+        if (!last && lane < C) ptx::mbar_arrive_remote(ptx::map_to_rank(rempty_bar, lane));
+      };
+      // Before this warp lays out anything: every rank has read the exchange before (and with
+      // that, the copies out of this warp's layout are done).
+      auto layout_free = [&]() {
+        ok = ptx::mbar_wait_acquire_cluster(rempty_bar, (uint32_t)(xc & 1) ^ 1u, abort_flag, p.wait_ns);
+        ok = __all_sync(0xffffffffu, ok);
+      };
+      // 16 tokens' sums of this lane's weight row: finished here, or laid out (and exchanged
+      // when the layout is full or the tile ends)
       auto emit = [&](int c, const uint32_t (&r)[16]) {
         if constexpr (!SPLIT) {
           with_act(ep.act, [&](auto act) {
             finish_chunk<KIND, GATED, decltype(act)::value>(ep, fl, t.t0 + c, t.n - c, lane, r, [] {});
           });
         } else {
+          const int x0 = c / XT * XT;
+          if (c == x0) layout_free();
+          if (!ok) return;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            if (c + j < t.n) {
-              ptx::st_async_u32(to, r[j], to_bar);
-              to += WROWS * 4u;
-              if (++tl == per) {
-                tl = 0;
-                if (++dst < C) {
-                  to = ptx::map_to_rank(to0, dst);
-                  to_bar = ptx::map_to_rank(rfull_bar, dst);
-                }
-              }
-            }
-          }
+          for (int j = 0; j < 16; ++j)
+            st_shared_u32(send_q + (uint32_t)((c - x0 + j) * 32 + lane) * 4u, r[j]);
+          if (c + 16 >= t.n || c + 16 == x0 + XT) exchange(x0, min(t.n - x0, XT));
         }
       };
       float run[SEG ? strm::SEG_TOK / 16 : 1][16];
@@ -949,16 +1028,19 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
       for (int s0 = kb0; ok && s0 < kb1; s0 += seg, ++it) {
         const int a = it & 1;
         ok = ptx::mbar_wait(tfull_bar(a), (uint32_t)((it >> 1) & 1), abort_flag, p.wait_ns);
-        if (SPLIT && s0 + seg >= kb1)  // every rank has read the sums of the tile before
-          ok = ok && ptx::mbar_wait_acquire_cluster(rempty_bar, xphase ^ 1u, abort_flag, p.wait_ns);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         ptx::tc_fence_after();
         if constexpr (!SEG) {
-          for (int c = 0; c < t.n; c += 16) {
+          for (int c = 0; ok && c < t.n; c += 16) {
             uint32_t r[16];
             ptx::tmem_ld_32x32b_x16(tmem_q + (uint32_t)(a * TOK + c), r);
             ptx::tmem_wait_ld();
+            if (c + 16 >= t.n) {  // the accumulator is read: free before the last exchange
+              ptx::tc_fence_before();
+              __syncwarp();
+              if (lane == 0) ptx::mbar_arrive(tempty_bar(a));
+            }
             emit(c, r);
           }
         } else {
@@ -972,59 +1054,23 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
               for (int j = 0; j < 16; ++j)
                 run[i][j] = s0 == kb0 ? __uint_as_float(r[j]) : __fadd_rn(run[i][j], __uint_as_float(r[j]));
             }
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(tempty_bar(a));
         }
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(tempty_bar(a));
-      }
-      if (!ok) {
-        if (lane == 0 && !*abort_flag) report_cluster(p.err, DEVERR_TIMEOUT_EPILOGUE, abort_flag, C);
-        break;
       }
       if constexpr (SEG) {
 #pragma unroll
         for (int i = 0; i < strm::SEG_TOK / 16; ++i)
-          if (16 * i < t.n) {
+          if (ok && 16 * i < t.n) {
             uint32_t r[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(run[i][j]);
             emit(16 * i, r);
           }
       }
-      if constexpr (SPLIT) {
-        ok = ptx::mbar_wait_acquire_cluster(rfull_bar, xphase, abort_flag, p.wait_ns);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) {
-          if (lane == 0 && !*abort_flag) report_cluster(p.err, DEVERR_TIMEOUT_EPILOGUE, abort_flag, C);
-          break;
-        }
-        if (last_tile) {  // this warp has made its last access to another CTA
-          ptx::cluster_arrive();
-          arrived = true;
-        }
-        // words of this lane's four features in a token's 128: gated, gate rows then up rows
-        // by turns of 16
-        const int at0 = GATED ? (lane % 16) / 4 * 32 + (lane % 4) * 4 : 4 * lane;
-        with_act(ep.act, [&](auto act) {
-          for (int l = GATED ? (warp - 2) * 2 + lane / 16 : warp - 2; l < mine; l += GATED ? 8 : 4) {
-            const int row = t.t0 + rank * per + l;
-            if (ff.n >= ep.N) continue;
-            float sx = 1.f, res[4];
-            if (KIND == KIND_I8) sx = __ldg(ep.sx + row);
-            load_residual(ep, row, ff.n, res);
-            uint32_t g[4] = {0u, 0u, 0u, 0u}, u[4] = {0u, 0u, 0u, 0u};
-            for (int c = 0; c < C; ++c) {
-              const uint32_t at = recv + (uint32_t)((c * slot + l) * WROWS + at0) * 4u;
-              add_words<KIND>(g, ld_shared_v4(at));
-              if (GATED) add_words<KIND>(u, ld_shared_v4(at + 16 * 4));
-            }
-            finish4<KIND, GATED, decltype(act)::value>(ep, ff, row, sx, g, u, res);
-          }
-        });
-        __syncwarp();
-        if (!last_tile && lane < C)
-          ptx::mbar_arrive_release_cluster(ptx::map_to_rank(rempty_bar, lane));
-      }
+      if (!ok && lane == 0 && !*abort_flag)
+        report_cluster(p.err, DEVERR_TIMEOUT_EPILOGUE, abort_flag, C);
     }
     if (SPLIT && !arrived) {
       __syncwarp();
@@ -1077,15 +1123,16 @@ static bool make_map(CUtensorMap* m, const void* ptr, uint64_t width, uint64_t r
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// The gated weights [E][2][N][K] as (k, row of 16, gate / up, block of 16 features, expert);
-// features past the last whole block are outside the map.  Boxes of 128 bytes x 16 rows x both
-// halves x 4 blocks: 128 weight rows, gate and up interleaved by 16.
-static bool make_gated_map(CUtensorMap* m, const void* ptr, uint64_t width, int N, int E) {
+// The gated weights [E][2][N][K] as (k, row of 8, gate / up, block of 8 features, expert);
+// features past the last whole block are outside the map.  Boxes of 128 bytes x 8 rows x both
+// halves x `blocks` blocks: 16 * blocks weight rows, gate and up by turns of 8.
+static bool make_gated_map(CUtensorMap* m, const void* ptr, uint64_t width, int N, int E,
+                           int blocks) {
   EncodeTiledFn enc = encode_fn();
   if (!enc) return false;
-  cuuint64_t dims[5] = {width, 16, 2, (cuuint64_t)(N / 16), (cuuint64_t)E};
-  cuuint64_t strides[4] = {width, (cuuint64_t)N * width, 16 * width, 2 * (cuuint64_t)N * width};
-  cuuint32_t box[5] = {BK, 16, 2, 4, 1};
+  cuuint64_t dims[5] = {width, 8, 2, (cuuint64_t)(N / 8), (cuuint64_t)E};
+  cuuint64_t strides[4] = {width, (cuuint64_t)N * width, 8 * width, 2 * (cuuint64_t)N * width};
+  cuuint32_t box[5] = {BK, 8, 2, (cuuint32_t)blocks, 1};
   cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, const_cast<void*>(ptr), dims, strides, box,
              estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -1200,23 +1247,15 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
   p.num_k_blocks = (int)(((long long)a.K * es + BK - 1) / BK);
   p.err = s->dev->d_err;
   p.wait_ns = s->dev->wait_ns;
-  p.feats = a.gated ? 64 : 128;
+  p.rows = WROWS;
   const int table = ((3 * a.E + 1) * 4 + 15) / 16 * 16;
   // rows of a group if they are spread evenly; the kernels take any spread
   const int groups = a.E < a.M ? a.E : a.M;
   const int avg = (a.M + groups - 1) / groups;
   const bool use_pair = avg > 128;
-  // rows of a weight box: all of a CTA's, or a run of gate or up rows
-  const int w_rows = a.gated ? 16 : WROWS;
   p.seg_kb = SEG_KB;
   const bool seg = a.kind == KIND_BF16 && a.out_dtype == QGEMM_F32 && p.num_k_blocks > SEG_KB;
   const int variant = a.kind == KIND_I8 ? 0 : seg ? 2 : 1;
-  CUtensorMap tmW, tmG, tmX;
-  memset(&tmG, 0, sizeof(tmG));
-  if (a.gated && a.N >= 64 && !make_gated_map(&tmG, a.w, (uint64_t)a.K * es, a.N, a.E))
-    return fail(QGEMM_ERR_CUDA, "cuTensorMapEncodeTiled failed for the gated weights");
-  if (!make_map(&tmW, a.w, (uint64_t)a.K * es, (uint64_t)a.E * p.ep.nw, (uint64_t)a.K * es, w_rows))
-    return fail(QGEMM_ERR_CUDA, "cuTensorMapEncodeTiled failed for the weights");
   cudaLaunchConfig_t cfg = {};
   cfg.stream = s->stream;
   cudaLaunchAttribute attr[2];
@@ -1235,6 +1274,7 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
     const long long block_bytes = (long long)p.tok_max * a.K * es;
     p.band = (int)(block_bytes > (48 << 20) ? 1 : (48 << 20) / block_bytes);
     p.tok_round = 32;
+    p.feats = a.gated ? 64 : 128;
     p.num_w_blocks = (a.N + 2 * p.feats - 1) / (2 * p.feats);
     box = 128;
     const int fixed = BAR_BYTES + table + 1024;
@@ -1249,23 +1289,37 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
     p.tok_max = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 || seg ? 64 : 128;
     p.tok_round = 16;
     p.band = 1 << 20;  // token blocks run fastest: neighbours share the weights
-    p.num_w_blocks = (a.N + p.feats - 1) / p.feats;
     box = p.tok_max < 32 ? p.tok_max : 32;
-    // Cut of K: rounds of tiles over the clusters that fit, times the k-blocks of a part,
-    // plus a part's fixed cost (pipeline fill and exchange, about 3 k-blocks' time).
-    const long long tiles = (long long)p.num_w_blocks * groups * ((avg + p.tok_max - 1) / p.tok_max);
+    // Cut of the work: K over c CTAs, and weight rows a tile, so that the rounds come out full.
+    // Model, from timings of 4096 and 11008 features x 4096 at 1 to 128 tokens: a k-block costs
+    // its rows' share of what one CTA's copies bring in (48 GB/s when all stream) or the floor
+    // of its barriers and MMAs; a part of K an exchange at its end.
+    const long long groups_tok = (long long)groups * ((avg + p.tok_max - 1) / p.tok_max);
+    const int tok_rows = (((avg < p.tok_max ? avg : p.tok_max) + box - 1) / box) * box;
     double best = 0;
     int pick = 0;
     for (int i = 0; i < 4; ++i) {
       const int c = 1 << i;
       if (ds->clusters[i] < 1 || c > p.num_k_blocks) continue;
-      const long long rounds = (tiles + ds->clusters[i] - 1) / ds->clusters[i];
-      const double cost = (double)rounds * ((p.num_k_blocks + c - 1) / c + (c > 1 ? 3 : 1));
-      if (best == 0 || cost < best) { best = cost; pick = i; }
+      for (int r = WROWS; r >= 16; r -= 16) {
+        const int feats = a.gated ? r / 2 : r;
+        const long long tiles = groups_tok * ((a.N + feats - 1) / feats);
+        const long long rounds = (tiles + ds->clusters[i] - 1) / ds->clusters[i];
+        double kb_us = (r + 0.5 * tok_rows) * BK / 48e3;
+        if (kb_us < 0.12) kb_us = 0.12;
+        const double us = rounds * (((p.num_k_blocks + c - 1) / c) * kb_us + 0.2) +
+                          (c > 1 ? 1.0 + 0.02 * tok_rows : 0.0);
+        if (best == 0 || us < 0.98 * best) { best = us; pick = i; p.rows = r; }
+      }
     }
     p.csize = 1 << pick;
-    const int stage = W_BYTES + p.tok_max * BK;
-    const int fixed = (p.csize > 1 ? p.tok_max * WROWS * 4 : 0) + BAR_BYTES + table + 1024;
+    p.feats = a.gated ? p.rows / 2 : p.rows;
+    p.num_w_blocks = (a.N + p.feats - 1) / p.feats;
+    const int stage = (p.rows + p.tok_max) * BK;
+    const int xt = p.tok_max < strm::XTOK ? p.tok_max : strm::XTOK;
+    // the last stage's MMAs read a whole weight tile, past the ring if rows is small
+    const int fixed = (p.csize > 1 ? 2 * xt * WROWS * 4 : 0) + BAR_BYTES + table + 1024 +
+                      (stage < W_BYTES ? W_BYTES - stage : 0);
     p.stages = (SMEM_MAX - fixed) / stage;
     if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
     cfg.dynamicSmemBytes = (size_t)fixed + (size_t)p.stages * stage;
@@ -1282,6 +1336,15 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
     attr[1].val.clusterDim.z = 1;
     cfg.numAttrs = 2;
   }
+  // weight boxes: all of a CTA's rows, or (gated) runs of 8 and the 5-D map over them
+  CUtensorMap tmW, tmG, tmX;
+  memset(&tmG, 0, sizeof(tmG));
+  if (!make_map(&tmW, a.w, (uint64_t)a.K * es, (uint64_t)a.E * p.ep.nw, (uint64_t)a.K * es,
+                a.gated ? 8 : p.rows))
+    return fail(QGEMM_ERR_CUDA, "cuTensorMapEncodeTiled failed for the weights");
+  if (a.gated && a.N / 8 >= p.rows / 16 &&
+      !make_gated_map(&tmG, a.w, (uint64_t)a.K * es, a.N, a.E, p.rows / 16))
+    return fail(QGEMM_ERR_CUDA, "cuTensorMapEncodeTiled failed for the gated weights");
   if (!make_map(&tmX, a.x, (uint64_t)a.K * es, (uint64_t)a.M, (uint64_t)a.ldx * es, box))
     return fail(QGEMM_ERR_CUDA, "cuTensorMapEncodeTiled failed for x");
   CUtensorMap tmXs;

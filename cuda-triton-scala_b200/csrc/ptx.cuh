@@ -70,6 +70,20 @@ __device__ __forceinline__ bool mbar_try_wait_sleep(uint32_t bar, uint32_t parit
   return ok != 0;
 }
 
+// True in one lane of a converged warp (the same one every time).  A loop that a whole warp
+// walks with the copies and MMAs under this predicate keeps its addresses and descriptors in
+// uniform registers; the same loop inside `if (lane == 0)` took 630 cycles for a k-block's four
+// MMAs and barriers, 2.4 times the tensor pipe's need.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
 // Bounded wait that sleeps between polls (for warps that have nothing else to do).
 __device__ __forceinline__ bool mbar_wait_sleep(uint32_t bar, uint32_t parity,
                                                 const volatile int* abort,
@@ -238,21 +252,16 @@ __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
-// As above with release semantics at cluster scope: orders the thread's (and, after a
-// __syncwarp, its warp's) writes to any shared memory of the cluster before the arrival.
-__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
-               : "memory");
-}
-
-// One word to shared memory anywhere in the cluster, counted (4 bytes) on an mbarrier of the
-// same CTA as the destination: both addresses from map_to_rank of one rank.
-__device__ __forceinline__ void st_async_u32(uint32_t cluster_addr, uint32_t v,
-                                             uint32_t cluster_bar) {
-  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.u32 [%0], %1, [%2];" ::"r"(
-                   cluster_addr),
-               "r"(v), "r"(cluster_bar)
-               : "memory");
+// Bulk copy from this CTA's shared memory to shared memory anywhere in the cluster, counted in
+// bytes on an mbarrier of the destination's CTA (addresses from map_to_rank; 16-byte aligned,
+// size a multiple of 16).
+__device__ __forceinline__ void bulk_copy_cluster(uint32_t cluster_dst, uint32_t src, uint32_t bytes,
+                                                  uint32_t cluster_bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          cluster_dst),
+      "r"(src), "r"(bytes), "r"(cluster_bar)
+      : "memory");
 }
 
 // The two halves of cluster_sync_all.
@@ -268,8 +277,7 @@ __device__ __forceinline__ void st_cluster_u32(uint32_t cluster_addr, uint32_t v
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
 }
 
-// mbar_wait whose success acquires at cluster scope (pairs with
-// mbar_arrive_release_cluster on another CTA of the cluster).
+// mbar_wait whose success acquires at cluster scope (data that another CTA of the cluster sent).
 __device__ __forceinline__ bool mbar_wait_acquire_cluster(uint32_t bar, uint32_t parity,
                                                           const volatile int* abort,
                                                           unsigned long long limit_ns) {

@@ -435,3 +435,13 @@ def test_captured_and_replayed(gpu):
         d.check()
     del graphs
     st.destroy()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "w8a8"])
+@pytest.mark.parametrize("M", [1, 33])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("N", [17, 1500, 2501, 4800, 11008, 20002])
+def test_linear_few_rows_many_widths(gpu, kind, M, gated, N):
+    """Few rows: the weight rows a tile and the cut of K follow the width."""
+    run(gpu, Case(kind, M, N, 1040, act="silu", gated=gated, bias=True, residual=True),
+        qgemm.ALGO_TCGEN05)

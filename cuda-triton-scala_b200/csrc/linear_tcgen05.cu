@@ -62,8 +62,10 @@ struct Params {
   int rows;         // weight rows of a CTA's tile: 128, in the stream kernel a multiple of 16
   int feats;        // features of them: rows, gated rows / 2
   int stages;
-  int seg_kb;       // k-blocks summed in TMEM before the sums move to registers (SEG)
+  int seg_kb;       // k-blocks of one accumulator (SEG)
   int csize;        // CTAs of a cluster (stream kernel)
+  int box;          // token rows of a TMA box (stream kernel)
+  int tmem_cols;    // TMEM columns (stream kernel)
   int* err;
   unsigned long long wait_ns;
 };
@@ -387,6 +389,21 @@ __device__ __forceinline__ void finish_chunk(const Epi& ep, const Lane<GATED>& l
     finish_chunk_t<KIND, GATED, ACT, false>(ep, l, row0, n, lane, r, ready);
 }
 
+// SEG: r (16 fp32 accumulator columns being loaded) plus the running sums at TMEM address
+// `run` where `more` is set; valid after the call.
+__device__ __forceinline__ void add_running(uint32_t run, bool more, uint32_t (&r)[16]) {
+  if (more) {
+    uint32_t q[16];
+    ptx::tmem_ld_32x32b_x16(run, q);
+    ptx::tmem_wait_ld();
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      r[j] = __float_as_uint(__fadd_rn(__uint_as_float(q[j]), __uint_as_float(r[j])));
+  } else {
+    ptx::tmem_wait_ld();
+  }
+}
+
 // Calls fn with the activation as a compile-time constant.
 template <typename F>
 __device__ __forceinline__ void with_act(int act, F&& fn) {
@@ -653,8 +670,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
       const int chunks = (it_.n + CHUNK - 1) / CHUNK;
       // Waits for accumulator it & 1; a warp whose wait ran out stores nothing.
       auto acc_ready = [&]() {
-        bool ok = ptx::mbar_wait_sleep(tfull_bar(it & 1), (uint32_t)((it >> 1) & 1), abort_flag,
-                                       p.wait_ns);
+        bool ok = ptx::mbar_wait(tfull_bar(it & 1), (uint32_t)((it >> 1) & 1), abort_flag, p.wait_ns);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok && lane == 0 && !*abort_flag)
           report_cluster(p.err, DEVERR_TIMEOUT_EPILOGUE, abort_flag, 2);
@@ -667,53 +683,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
         if (lane == 0) ptx::mbar_arrive_remote((it & 1) ? te1 : te0);
         ++it;
       };
-      if constexpr (!SEG) {
+      // SEG: the running sums of the segments before live in TMEM columns 128 ..
+      const int seg = SEG ? p.seg_kb : p.num_k_blocks;
+      for (int kb = 0; kb < p.num_k_blocks; kb += seg) {
         const bool ok = acc_ready();
         const uint32_t acc = tmem_q + (uint32_t)((it & 1) * 256);
-        if (ok)
+        if (!ok) {
+        } else if (SEG && kb + seg < p.num_k_blocks) {
+          for (int c = grp; c < chunks; c += 2) {
+            uint32_t r[16];
+            ptx::tmem_ld_32x32b_x16(acc + (uint32_t)(c * CHUNK), r);
+            add_running(tmem_q + (uint32_t)(128 + c * CHUNK), kb > 0, r);
+            ptx::tmem_st_32x32b_x16(tmem_q + (uint32_t)(128 + c * CHUNK), r);
+          }
+          ptx::tmem_wait_st();
+        } else {
           with_act(p.ep.act, [&](auto act) {
             for (int c = grp; c < chunks; c += 2) {
               uint32_t r[16];
               ptx::tmem_ld_32x32b_x16(acc + (uint32_t)(c * CHUNK), r);
+              if (SEG) add_running(tmem_q + (uint32_t)(128 + c * CHUNK), kb > 0, r);
               finish_chunk<KIND, GATED, decltype(act)::value>(
-                  p.ep, f, it_.t0 + c * CHUNK, it_.n - c * CHUNK, lane, r, [] { ptx::tmem_wait_ld(); });
+                  p.ep, f, it_.t0 + c * CHUNK, it_.n - c * CHUNK, lane, r,
+                  [] { if (!SEG) ptx::tmem_wait_ld(); });
             }
           });
-        acc_done();
-      } else {
-        constexpr int MINE = pair::SEG_TOK / CHUNK / 2;  // chunks of a group
-        float run[MINE][16];
-        bool ok = true;
-        for (int kb = 0; kb < p.num_k_blocks; kb += p.seg_kb) {
-          ok = acc_ready() && ok;
-          const uint32_t acc = tmem_q + (uint32_t)((it & 1) * 256);
-#pragma unroll
-          for (int i = 0; i < MINE; ++i) {
-            const int c = grp + 2 * i;
-            if (ok && c < chunks) {
-              uint32_t r[16];
-              ptx::tmem_ld_32x32b_x16(acc + (uint32_t)(c * CHUNK), r);
-              ptx::tmem_wait_ld();
-#pragma unroll
-              for (int j = 0; j < 16; ++j)
-                run[i][j] = kb == 0 ? __uint_as_float(r[j]) : __fadd_rn(run[i][j], __uint_as_float(r[j]));
-            }
-          }
-          acc_done();
         }
-        if (ok)
-          with_act(p.ep.act, [&](auto act) {
-#pragma unroll
-            for (int i = 0; i < MINE; ++i) {
-              const int c = grp + 2 * i;
-              if (c >= chunks) continue;
-              uint32_t r[16];
-#pragma unroll
-              for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(run[i][j]);
-              finish_chunk<KIND, GATED, decltype(act)::value>(
-                  p.ep, f, it_.t0 + c * CHUNK, it_.n - c * CHUNK, lane, r, [] {});
-            }
-          });
+        acc_done();
       }
     }
   }
@@ -729,10 +725,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
 }
 
 // ---- the streaming kernel ------------------------------------------------------------------
-namespace strm {  // tiles of 16, 32, 64 or 128 tokens at most (Params::tok_max)
+namespace strm {  // tiles of 16 to 96 tokens at most (Params::tok_max, a multiple of 16)
 constexpr int THREADS = 192;   // producer, MMA issuer, four epilogue warps
-constexpr int SEG_TOK = 64;    // tokens of a tile at most with SEG
+constexpr int SEG_TOK = 64;    // tokens of a tile at most with SEG: three times as many columns
 constexpr int XTOK = 64;       // tokens of an exchange at most (SPLIT)
+constexpr int STEP = 2;        // k-blocks of a stage: one barrier round for both
 }  // namespace strm
 
 // SPLIT: a cluster of csize CTAs cuts K.  The sums of a token go to the rank that finishes it,
@@ -751,9 +748,10 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
   const uint32_t base = (raw_base + 1023u) & ~1023u;
   uint8_t* gbase = smem_raw + (base - raw_base);
   const int S = p.stages, TOK = p.tok_max, C = SPLIT ? p.csize : 1;
-  const int box = TOK < 32 ? TOK : 32;  // token rows of a TMA box
+  const int box = p.box;
   const uint32_t w_bytes = (uint32_t)(p.rows * BK);
-  const uint32_t stage_bytes = w_bytes + (uint32_t)(TOK * BK);
+  const uint32_t x_bytes = (uint32_t)(TOK * BK);
+  const uint32_t stage_bytes = strm::STEP * (w_bytes + x_bytes);  // weights, then tokens
   // SPLIT: the sums that this rank sends, [warp][token][32 weight rows] words, and those of its
   // own tokens, [source rank][warp][XT / C tokens][32]
   const int XT = min(TOK, strm::XTOK);
@@ -778,7 +776,7 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int rank = SPLIT ? (int)ptx::cluster_ctarank() : 0;
   const int cid = blockIdx.x / C, nclusters = gridDim.x / C;
-  const uint32_t tmem_cols = 2u * TOK;  // 32, 64, 128 or 256
+  const uint32_t tmem_cols = (uint32_t)p.tmem_cols;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
@@ -811,8 +809,10 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
   if (p.offsets) fill_table(p, tb);
   const uint32_t tmem_base = *tmem_slot;
   const int T = tb.pref[p.E];
-  const int kb0 = (int)((long long)p.num_k_blocks * rank / C);
-  const int kb1 = (int)((long long)p.num_k_blocks * (rank + 1) / C);
+  // this rank's k-blocks: whole stages, at least one (the host cuts K no finer)
+  const int ksteps = (p.num_k_blocks + strm::STEP - 1) / strm::STEP;
+  const int kb0 = ksteps * rank / C * strm::STEP;
+  const int kb1 = min(p.num_k_blocks, ksteps * (rank + 1) / C * strm::STEP);
 
   if (warp == 0) {
     // ---------------- TMA producer ----------------
@@ -825,29 +825,40 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
       const int boxes = (t.n + box - 1) / box;
       const uint32_t tx = w_bytes + (uint32_t)(boxes * box * BK);
       const int f0 = t.wb * p.feats, w0 = t.e * p.ep.nw + f0;
-      for (int kb = kb0; kb < kb1; ++kb) {
+      for (int kb = kb0; kb < kb1; kb += strm::STEP) {
         if (!warp_wait(p, empty_bar(stage), phase ^ 1u, abort_flag, DEVERR_TIMEOUT_PRODUCER, C)) {
           ok = false;
           break;
         }
         if (ptx::elect_one()) {
-          const uint32_t sw = base + stage * stage_bytes, sx = sw + w_bytes;
           const uint32_t fb = full_bar(stage);
-          ptx::mbar_arrive_expect_tx(fb, tx);
-          if constexpr (GATED) {  // gate and up rows by turns of 8, as in the pair kernel
-            if (f0 + p.feats <= p.ep.N / 8 * 8) {
-              ptx::tma_load_5d(sw, &tmG, fb, kb * BK, 0, 0, f0 / 8, t.e);
-            } else {
-              for (int b = 0; b < p.feats / 8; ++b) {
-                ptx::tma_load_2d(sw + (2 * b) * 8 * BK, &tmW, fb, kb * BK, w0 + 8 * b);
-                ptx::tma_load_2d(sw + (2 * b + 1) * 8 * BK, &tmW, fb, kb * BK, w0 + p.ep.N + 8 * b);
+          const int nk = min(strm::STEP, kb1 - kb);
+          ptx::mbar_arrive_expect_tx(fb, (uint32_t)nk * tx);
+#pragma unroll
+          for (int h = 0; h < strm::STEP; ++h) {
+            if (h >= nk) break;
+            const uint32_t sw = base + stage * stage_bytes + h * w_bytes;
+            const int ck = (kb + h) * BK;
+            if constexpr (GATED) {  // gate and up rows by turns of 8, as in the pair kernel
+              if (f0 + p.feats <= p.ep.N / 8 * 8) {
+                ptx::tma_load_5d(sw, &tmG, fb, ck, 0, 0, f0 / 8, t.e);
+              } else {
+                for (int b = 0; b < p.feats / 8; ++b) {
+                  ptx::tma_load_2d(sw + (2 * b) * 8 * BK, &tmW, fb, ck, w0 + 8 * b);
+                  ptx::tma_load_2d(sw + (2 * b + 1) * 8 * BK, &tmW, fb, ck, w0 + p.ep.N + 8 * b);
+                }
               }
+            } else {
+              ptx::tma_load_2d(sw, &tmW, fb, ck, w0);
             }
-          } else {
-            ptx::tma_load_2d(sw, &tmW, fb, kb * BK, w0);
           }
-          for (int b = 0; b < boxes; ++b)
-            ptx::tma_load_2d(sx + b * box * BK, &tmX, fb, kb * BK, t.t0 + b * box);
+#pragma unroll
+          for (int h = 0; h < strm::STEP; ++h) {
+            if (h >= nk) break;
+            const uint32_t sx = base + stage * stage_bytes + strm::STEP * w_bytes + h * x_bytes;
+            for (int b = 0; b < boxes; ++b)
+              ptx::tma_load_2d(sx + b * box * BK, &tmX, fb, (kb + h) * BK, t.t0 + b * box);
+          }
         }
         __syncwarp();
         ++issued;
@@ -886,7 +897,7 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
         ptx::tc_fence_after();
         const uint32_t d_tmem = tmem_base + (uint32_t)(a * TOK);
         const int s1 = min(s0 + seg, kb1);
-        for (int kb = s0; kb < s1; ++kb) {
+        for (int kb = s0; kb < s1; kb += strm::STEP) {
           if (!warp_wait(p, full_bar(stage), phase, abort_flag, DEVERR_TIMEOUT_MMA, C)) {
             ok = false;
             break;
@@ -896,18 +907,23 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
             // the MMA reads 128 weight rows: past p.rows they are whatever the ring holds, and
             // only lanes that nothing reads see them
             const uint32_t sw = base + stage * stage_bytes;
-            const uint64_t adesc = ptx::smem_desc_sw128(sw, 16, 1024);
-            const uint64_t bdesc = ptx::smem_desc_sw128(sw + w_bytes, 16, 1024);
+            const int nk = min(strm::STEP, s1 - kb);
 #pragma unroll
-            for (int kk = 0; kk < BK / UMMA_K; ++kk) {
-              const uint32_t accum = (kb != s0 || kk != 0) ? 1u : 0u;
-              if constexpr (KIND == KIND_BF16)
-                ptx::umma_bf16(d_tmem, adesc + kk * (UMMA_K / 16), bdesc + kk * (UMMA_K / 16), idesc, accum);
-              else
-                ptx::umma_i8(d_tmem, adesc + kk * (UMMA_K / 16), bdesc + kk * (UMMA_K / 16), idesc, accum);
+            for (int h = 0; h < strm::STEP; ++h) {
+              if (h >= nk) break;
+              const uint64_t adesc = ptx::smem_desc_sw128(sw + h * w_bytes, 16, 1024);
+              const uint64_t bdesc = ptx::smem_desc_sw128(sw + strm::STEP * w_bytes + h * x_bytes, 16, 1024);
+#pragma unroll
+              for (int kk = 0; kk < BK / UMMA_K; ++kk) {
+                const uint32_t accum = (kb != s0 || h != 0 || kk != 0) ? 1u : 0u;
+                if constexpr (KIND == KIND_BF16)
+                  ptx::umma_bf16(d_tmem, adesc + kk * (UMMA_K / 16), bdesc + kk * (UMMA_K / 16), idesc, accum);
+                else
+                  ptx::umma_i8(d_tmem, adesc + kk * (UMMA_K / 16), bdesc + kk * (UMMA_K / 16), idesc, accum);
+              }
             }
             ptx::umma_commit(empty_bar(stage));
-            if (kb + 1 == s1) ptx::umma_commit(tfull_bar(a));
+            if (kb + nk >= s1) ptx::umma_commit(tfull_bar(a));
           }
           __syncwarp();
           issued_any = true;
@@ -1023,7 +1039,7 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
           if (c + 16 >= t.n || c + 16 == x0 + XT) exchange(x0, min(t.n - x0, XT));
         }
       };
-      float run[SEG ? strm::SEG_TOK / 16 : 1][16];
+      // SEG: the running sums of the segments before live in TMEM columns 2 TOK ..
       const int seg = SEG ? p.seg_kb : p.num_k_blocks;
       for (int s0 = kb0; ok && s0 < kb1; s0 += seg, ++it) {
         const int a = it & 1;
@@ -1031,43 +1047,21 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         ptx::tc_fence_after();
-        if constexpr (!SEG) {
-          for (int c = 0; ok && c < t.n; c += 16) {
-            uint32_t r[16];
-            ptx::tmem_ld_32x32b_x16(tmem_q + (uint32_t)(a * TOK + c), r);
-            ptx::tmem_wait_ld();
-            if (c + 16 >= t.n) {  // the accumulator is read: free before the last exchange
-              ptx::tc_fence_before();
-              __syncwarp();
-              if (lane == 0) ptx::mbar_arrive(tempty_bar(a));
-            }
-            emit(c, r);
+        const bool last_seg = !SEG || s0 + seg >= kb1;
+        for (int c = 0; ok && c < t.n; c += 16) {
+          uint32_t r[16];
+          ptx::tmem_ld_32x32b_x16(tmem_q + (uint32_t)(a * TOK + c), r);
+          if (SEG) add_running(tmem_q + (uint32_t)(2 * TOK + c), s0 > kb0, r);
+          else ptx::tmem_wait_ld();
+          if (!last_seg) ptx::tmem_st_32x32b_x16(tmem_q + (uint32_t)(2 * TOK + c), r);
+          if (c + 16 >= t.n) {  // the accumulator is read: free before the last exchange
+            if (SEG) ptx::tmem_wait_st();
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(tempty_bar(a));
           }
-        } else {
-#pragma unroll
-          for (int i = 0; i < strm::SEG_TOK / 16; ++i)
-            if (16 * i < t.n) {
-              uint32_t r[16];
-              ptx::tmem_ld_32x32b_x16(tmem_q + (uint32_t)(a * TOK + 16 * i), r);
-              ptx::tmem_wait_ld();
-#pragma unroll
-              for (int j = 0; j < 16; ++j)
-                run[i][j] = s0 == kb0 ? __uint_as_float(r[j]) : __fadd_rn(run[i][j], __uint_as_float(r[j]));
-            }
-          ptx::tc_fence_before();
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(tempty_bar(a));
+          if (last_seg) emit(c, r);
         }
-      }
-      if constexpr (SEG) {
-#pragma unroll
-        for (int i = 0; i < strm::SEG_TOK / 16; ++i)
-          if (ok && 16 * i < t.n) {
-            uint32_t r[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(run[i][j]);
-            emit(16 * i, r);
-          }
       }
       if (!ok && lane == 0 && !*abort_flag)
         report_cluster(p.err, DEVERR_TIMEOUT_EPILOGUE, abort_flag, C);
@@ -1154,12 +1148,16 @@ static const Kern kStream[3][2][2] = {
     {{linear_stream_kernel<KIND_BF16, false, true, false>, linear_stream_kernel<KIND_BF16, false, true, true>},
      {linear_stream_kernel<KIND_BF16, true, true, false>, linear_stream_kernel<KIND_BF16, true, true, true>}}};
 
+static_assert(pair::SEG_TOK <= 128 && 3 * strm::SEG_TOK <= 256, "TMEM columns of SEG");
+
 // The tensor cores add each MMA's products to the fp32 accumulator by truncation, so a sum
 // over K shrinks by about 9e-10 of itself a value of K (measured: 2.1e-6 at K = 2048, 1.2e-5 at
-// 11008).  bf16 outputs round 300 times coarser; fp32 outputs take the SEG kernels, which move
-// the accumulator to registers every SEG_KB k-blocks (512 values, 4.7e-7) and add the pieces
-// rounding to nearest.
+// 11008).  bf16 outputs round 300 times coarser; fp32 outputs take the SEG kernels, which start
+// a new accumulator every SEG_KB k-blocks (512 values, 4.7e-7) and add the pieces rounding to
+// nearest, into running sums in TMEM (in registers, the unrolled code ran from outside the
+// instruction cache: 170 us instead of 112 for 6001 x 1544 x 2048 over 64 experts).
 constexpr int SEG_KB = 8;
+static_assert(SEG_KB % strm::STEP == 0, "a segment is whole stages");
 
 // Opts the kernels in to the whole shared memory once a device, and asks how many clusters of
 // 1, 2, 4 and 8 streaming CTAs the device holds at once.
@@ -1252,10 +1250,79 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
   // rows of a group if they are spread evenly; the kernels take any spread
   const int groups = a.E < a.M ? a.E : a.M;
   const int avg = (a.M + groups - 1) / groups;
-  const bool use_pair = avg > 128;
   p.seg_kb = SEG_KB;
   const bool seg = a.kind == KIND_BF16 && a.out_dtype == QGEMM_F32 && p.num_k_blocks > SEG_KB;
   const int variant = a.kind == KIND_I8 ? 0 : seg ? 2 : 1;
+  // ---- the streaming kernel's cut of the work ----
+  const int cap = seg ? strm::SEG_TOK : 96;  // 96: more tokens leave too few stages
+  int tok_max, box;
+  if (a.offsets) {
+    // tokens of a tile: twice the even share, so that a moderate skew stays in one tile
+    const int want = 2 * avg < a.M ? 2 * avg : a.M;
+    tok_max = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : cap;
+    box = tok_max < 32 ? tok_max : 32;
+  } else {  // equal blocks, each one box
+    const int nblk = (a.M + cap - 1) / cap;
+    tok_max = ((a.M + nblk - 1) / nblk + 15) / 16 * 16;
+    box = tok_max;
+  }
+  // K over c CTAs, and weight rows a tile, so that the rounds come out full.  A round takes the
+  // longer of its k-blocks' copies and MMAs in a CTA (0.17 us each and more with more tokens,
+  // 0.22 gated) and of its weights from HBM (6.2 TB/s from all SMs), and a quarter of the
+  // other; a cut of K adds an exchange.  Measured against every choice at 9 shapes of 1024 to
+  // 11008 features and 1 to 100 tokens (1 x 4096 x 4096 bf16: 8.9 us with c = 4, 10.1 with 2,
+  // 14.7 with 1; 33 x 11008 x 4096 int8 gated: 21.2 us with c = 2 and 112 rows, 22.5 with c = 1
+  // and 128).
+  const int ksteps = (p.num_k_blocks + strm::STEP - 1) / strm::STEP;
+  const long long groups_tok = (long long)groups * ((avg + tok_max - 1) / tok_max);
+  const double tok = avg < tok_max ? avg : tok_max;
+  const double kb_us = (a.gated ? 0.22 : 0.17) + 0.0009 * tok;
+  auto both = [](double x, double y) { return x > y ? x + 0.25 * y : y + 0.25 * x; };
+  // a stage holds tok_max token rows and is filled in whole boxes
+  if (tok_max % box != 0 || tok_max > 96 || box > 128)
+    return fail(QGEMM_ERR_UNSUPPORTED, "token tile %d in boxes of %d", tok_max, box);
+  double stream_us = 0;
+  int pick = 0, rows = WROWS;
+  for (int i = 0; i < 4; ++i) {
+    const int c = 1 << i;
+    if (ds->clusters[i] < 1 || c > ksteps) continue;
+    for (int r = WROWS; r >= 64; r -= 16) {
+      // fewer rows a tile pay only where the counts are known and the epilogue is short (6001
+      // rows over 64 experts, fp32 out: 100 us with 128 rows, 118 with 112)
+      if (r < WROWS && (a.offsets || tok > 64)) continue;
+      const int feats = a.gated ? r / 2 : r;
+      const long long tiles = groups_tok * ((a.N + feats - 1) / feats);
+      // a cut of K only where tiles are scarce: with many, its exchange is paid for every one
+      // (those 6001 rows: 208 us with c = 2, 108 with c = 1)
+      if (c > 1 && tiles >= 2 * sms) continue;
+      const long long full = tiles / ds->clusters[i], rest = tiles - full * ds->clusters[i];
+      double cta = (ksteps + c - 1) / c * strm::STEP * kb_us + 0.1;
+      if (c > 1 && cta < 1.2 + 0.03 * tok) cta = 1.2 + 0.03 * tok;  // an exchange a tile
+      const int ctas = c * ds->clusters[i];
+      const double tile_hbm = (double)r * a.K * es / (6.2e6 * (ctas < sms ? ctas : sms) / sms);
+      const double us = (r < WROWS ? 1.03 : 1.0) * (full * both(cta, ds->clusters[i] * tile_hbm) +
+                        (rest ? both(cta, rest * tile_hbm) : 0.0)) + (c > 1 ? 0.6 + 0.05 * tok : 0.0);
+      if (stream_us == 0 || us < stream_us) { stream_us = us; pick = i; rows = r; }
+    }
+  }
+  // ---- the pair kernel's time, in the same terms ----
+  const int pair_feats = a.gated ? 128 : 256, pair_tok = seg ? pair::SEG_TOK : pair::TOK;
+  const int pairs = sms / 2;
+  const long long pair_blocks = (avg + pair_tok - 1) / pair_tok;
+  const long long pair_tiles = groups * pair_blocks * ((a.N + pair_feats - 1) / pair_feats);
+  const double pair_n = (double)avg / pair_blocks;
+  auto pair_round = [&](long long n, double toks) {
+    return p.num_k_blocks * both(0.24 + 0.0005 * toks, n * 2 * W_BYTES / 6.2e6);
+  };
+  const long long pfull = pair_tiles / pairs, prest = pair_tiles - pfull * pairs;
+  // (SEG costs the pair kernel half its time more: 142 us against 100 streaming for those rows)
+  const double pair_us = 0.5 + (seg ? 1.5 : 1.0) * pfull * pair_round(pairs, pair_n) +
+      (prest ? (seg ? 1.5 : 1.0) * pair_round(prest, pair_n / (pairs / prest < 4 ? pairs / prest : 4)) : 0.0);
+  // Which kernel: the model where a group has up to 96 rows (measured, bf16 4096 x 4096: 64 rows
+  // 12.2 us streaming, 19.5 in pairs; 128 rows 17.7 and 19.9; 256 rows 24.6 and 20.9; 11008 x
+  // 4096: 96 rows 22.6 and 24.8; 128 rows 34.9 and 25.6).
+  const bool use_pair = avg > 96 || pair_us < stream_us;
+
   cudaLaunchConfig_t cfg = {};
   cfg.stream = s->stream;
   cudaLaunchAttribute attr[2];
@@ -1264,9 +1331,8 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   Kern kern;
-  int box;
   if (use_pair) {
-    p.tok_max = seg ? pair::SEG_TOK : pair::TOK;
+    p.tok_max = pair_tok;
     // A band's tokens stay in L2 while all weights pass by once: the fewer bands, the fewer
     // times the weights come from HBM, whose power the tensor cores then lack (int8 8192 x
     // 28672 x 4096: 805 us with 32 MB of tokens a band, 815 with 16, 825 with 8; bf16 4096 x
@@ -1284,48 +1350,27 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
     cfg.blockDim = dim3(pair::THREADS);
     kern = kPair[variant][a.gated];
   } else {
-    // tokens of a tile: twice the even share, so that a moderate skew stays in one tile
-    const int want = a.offsets ? (2 * avg < a.M ? 2 * avg : a.M) : a.M;
-    p.tok_max = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 || seg ? 64 : 128;
+    p.tok_max = tok_max;
+    p.box = box;
+    const int cols = (seg ? 3 : 2) * tok_max;  // accumulators, running sums
+    p.tmem_cols = cols <= 32 ? 32 : cols <= 64 ? 64 : cols <= 128 ? 128 : 256;
     p.tok_round = 16;
     p.band = 1 << 20;  // token blocks run fastest: neighbours share the weights
-    box = p.tok_max < 32 ? p.tok_max : 32;
-    // Cut of the work: K over c CTAs, and weight rows a tile, so that the rounds come out full.
-    // Model, from timings of 4096 and 11008 features x 4096 at 1 to 128 tokens: a k-block costs
-    // its rows' share of what one CTA's copies bring in (48 GB/s when all stream) or the floor
-    // of its barriers and MMAs; a part of K an exchange at its end.
-    const long long groups_tok = (long long)groups * ((avg + p.tok_max - 1) / p.tok_max);
-    const int tok_rows = (((avg < p.tok_max ? avg : p.tok_max) + box - 1) / box) * box;
-    double best = 0;
-    int pick = 0;
-    for (int i = 0; i < 4; ++i) {
-      const int c = 1 << i;
-      if (ds->clusters[i] < 1 || c > p.num_k_blocks) continue;
-      for (int r = WROWS; r >= 16; r -= 16) {
-        const int feats = a.gated ? r / 2 : r;
-        const long long tiles = groups_tok * ((a.N + feats - 1) / feats);
-        const long long rounds = (tiles + ds->clusters[i] - 1) / ds->clusters[i];
-        double kb_us = (r + 0.5 * tok_rows) * BK / 48e3;
-        if (kb_us < 0.12) kb_us = 0.12;
-        const double us = rounds * (((p.num_k_blocks + c - 1) / c) * kb_us + 0.2) +
-                          (c > 1 ? 1.0 + 0.02 * tok_rows : 0.0);
-        if (best == 0 || us < 0.98 * best) { best = us; pick = i; p.rows = r; }
-      }
-    }
     p.csize = 1 << pick;
-    p.feats = a.gated ? p.rows / 2 : p.rows;
+    p.rows = rows;
+    p.feats = a.gated ? rows / 2 : rows;
     p.num_w_blocks = (a.N + p.feats - 1) / p.feats;
-    const int stage = (p.rows + p.tok_max) * BK;
-    const int xt = p.tok_max < strm::XTOK ? p.tok_max : strm::XTOK;
+    const int stage = strm::STEP * (rows + tok_max) * BK;
+    const int xt = tok_max < strm::XTOK ? tok_max : strm::XTOK;
     // the last stage's MMAs read a whole weight tile, past the ring if rows is small
     const int fixed = (p.csize > 1 ? 2 * xt * WROWS * 4 : 0) + BAR_BYTES + table + 1024 +
-                      (stage < W_BYTES ? W_BYTES - stage : 0);
+                      (stage < 2 * W_BYTES ? 2 * W_BYTES - stage : 0);
     p.stages = (SMEM_MAX - fixed) / stage;
     if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
     cfg.dynamicSmemBytes = (size_t)fixed + (size_t)p.stages * stage;
     // as many clusters as fit (the counts of the experts are not known here: at least one
     // tile each is not promised)
-    const long long most = (long long)p.num_w_blocks * (a.M / p.tok_max + groups);
+    const long long most = (long long)p.num_w_blocks * (a.M / tok_max + groups);
     const long long clusters = most < ds->clusters[pick] ? most : ds->clusters[pick];
     cfg.gridDim = dim3((unsigned)(clusters * p.csize));
     cfg.blockDim = dim3(strm::THREADS);

@@ -205,7 +205,9 @@ def check(status: int, func: str) -> None:
 
 def call(name: str, *args) -> None:
     """Calls an entry point and raises QGemmError on a non-OK status."""
-    check(getattr(lib(), name)(*args), name)
+    status = getattr(_lib or lib(), name)(*args)
+    if status != OK:
+        check(status, name)
 
 
 def try_call(name: str, *args) -> int:
@@ -218,10 +220,12 @@ def addr(x) -> int:
     Ptr.address), an object with ``.address`` or a torch tensor (data_ptr)."""
     if x is None:
         return 0
+    try:
+        return x.data_ptr()
+    except AttributeError:
+        pass
     if isinstance(x, int):
         return x
-    if hasattr(x, "data_ptr"):
-        return int(x.data_ptr())
     if hasattr(x, "address"):
         return int(x.address)
     raise TypeError(f"cannot take a device address of {type(x).__name__}")

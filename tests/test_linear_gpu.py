@@ -445,3 +445,37 @@ def test_linear_few_rows_many_widths(gpu, kind, M, gated, N):
     """Few rows: the weight rows a tile and the cut of K follow the width."""
     run(gpu, Case(kind, M, N, 1040, act="silu", gated=gated, bias=True, residual=True),
         qgemm.ALGO_TCGEN05)
+
+
+@pytest.mark.parametrize("avg", [20, 40, 94, 130])
+@pytest.mark.parametrize("gated", [False, True])
+def test_expert_linear_fp32_long_sums(gpu, avg, gated):
+    """fp32 outputs of more than 512 values a sum, over ragged groups around the kernels' token
+    tiles."""
+    rng = np.random.default_rng(avg)
+    off = np.concatenate([[0], np.cumsum(rng.integers(0, 2 * avg, 40))]).tolist()
+    run(gpu, Case("bf16", off[-1], 392, 1304, act="gelu_tanh", gated=gated, bias=True, out="f32",
+                  offsets=off))
+
+
+@pytest.mark.parametrize("M", [1, 63, 65, 81, 97, 200, 300])
+def test_linear_fp32_sums_keep_their_precision(gpu, M):
+    """Random bf16 operands, K = 8192, fp32 out: sums in pieces of 512 values.  A piece loses up
+    to one unit of the accumulator (2^-23 of the running sum, rounded toward zero) for each of
+    its 512 / 16 MMAs; the running sum never passes sum |x w|, so the error stays below
+    (32 + 16) 2^-23 of it (32 truncations a piece, 16 additions of pieces)."""
+    _, st, ops = gpu
+    N, K = 136, 8192
+    g = torch.Generator("cuda").manual_seed(M)
+    x = torch.randn(M, K, generator=g, device="cuda").bfloat16()
+    w = torch.randn(N, K, generator=g, device="cuda").bfloat16()
+    out = torch.empty(M, N, device="cuda")
+    torch.cuda.synchronize()
+    ops.linearBf16NK(x, w, out, M, N, K, out_dtype=qgemm.F32)
+    st.sync()
+    exact = x.double() @ w.double().t()
+    bound = 48 * 2.0 ** -23 * (x.double().abs() @ w.double().abs().t())
+    d = (out.double() - exact).abs()
+    assert (d <= bound).all()
+    # and in the mean far below what one accumulator over all of K loses (9e-6 of the result)
+    assert float(d.norm() / exact.norm()) < 2e-6

@@ -12,8 +12,6 @@
 namespace qg {
 namespace route {
 
-constexpr int WARPS = 32;           // warps of a grouping CTA
-constexpr int THREADS = 32 * WARPS;
 constexpr int CLUSTER = 8;          // grouping CTAs of a large call (portable cluster size)
 
 template <typename T> __device__ __forceinline__ float to_f(T v);
@@ -22,30 +20,54 @@ template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v
   return __bfloat162float(v);
 }
 
-// A key that orders like the float, 0 for what is never chosen (-inf, NaN).  -0 and +0 get
-// one key (they are equal, the lower index wins); +inf counts as the largest finite value.
-__device__ __forceinline__ uint32_t key_of(float v) {
-  if (!(v > -INFINITY)) return 0u;
-  v = fminf(v, FLT_MAX) + 0.0f;
-  const uint32_t b = __float_as_uint(v);
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-}
-__device__ __forceinline__ float value_of(uint32_t key) {
-  return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
-}
+// A key that orders like the logit, 0 for what is never chosen (-inf, NaN).  -0 and +0 get one
+// key (they are equal, the lower index wins); +inf counts as the largest finite fp32.  A bf16
+// logit leaves 16 bits for the (complemented) index, so one warp reduction finds the largest
+// and, among equals, the lowest index; fp32 logits need a second one for the index (at 16384
+// tokens, 64 experts and k = 8 the reductions are what bounds the kernel).
+template <typename T> struct Key;
+template <> struct Key<float> {
+  static constexpr bool kIndexed = false;
+  static __device__ __forceinline__ uint32_t of(float v, int) {
+    if (!(v > -INFINITY)) return 0u;
+    v = fminf(v, FLT_MAX) + 0.0f;
+    const uint32_t b = __float_as_uint(v);
+    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+  }
+  static __device__ __forceinline__ float value(uint32_t key) {
+    return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
+  }
+  static __device__ __forceinline__ int index(uint32_t) { return 0; }
+};
+template <> struct Key<__nv_bfloat16> {
+  static constexpr bool kIndexed = true;
+  static __device__ __forceinline__ uint32_t of(__nv_bfloat16 x, int e) {
+    float v = __bfloat162float(x);
+    if (!(v > -INFINITY)) return 0u;
+    v += 0.0f;
+    const uint32_t b = __float_as_uint(v) >> 16;
+    const uint32_t o = (b & 0x8000u) ? (~b & 0xffffu) : (b | 0x8000u);
+    return (o << 16) | (0xffffu - (uint32_t)e);
+  }
+  static __device__ __forceinline__ float value(uint32_t key) {
+    const uint32_t o = key >> 16;
+    return fminf(__uint_as_float(((o & 0x8000u) ? (o & 0x7fffu) : (~o & 0xffffu)) << 16), FLT_MAX);
+  }
+  static __device__ __forceinline__ int index(uint32_t key) { return (int)(0xffffu - (key & 0xffffu)); }
+};
 
 // One token by one warp: lane l holds the logits of experts l, l + 32, ...  Each round takes
-// the largest key of the warp (two warp reductions: the key, then the lowest index that has
-// it) and retires it; the softmax sum runs over the same registers.
+// the largest key of the warp and retires it; the softmax sum runs over the same registers.
 template <typename T, int EPL>
 __device__ __forceinline__ void topk_token(const T* __restrict__ logits, int E, int k,
                                            int renormalize, float* __restrict__ weights,
                                            int* __restrict__ experts, int lane) {
+  using K = Key<T>;
   uint32_t key[EPL];
 #pragma unroll
   for (int i = 0; i < EPL; ++i) {
     const int e = lane + 32 * i;
-    key[i] = e < E ? key_of(to_f<T>(logits[e])) : 0u;
+    key[i] = e < E ? K::of(logits[e], e) : 0u;
   }
   uint32_t best = 0;
   int at = 0;
@@ -58,22 +80,22 @@ __device__ __forceinline__ void topk_token(const T* __restrict__ logits, int E, 
   };
   rescan();
   const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-  const float most = value_of(top);
+  const float most = K::value(top);
   float sum = 0.f;  // over every expert that can be chosen
   if (!renormalize) {
 #pragma unroll
     for (int i = 0; i < EPL; ++i)
-      if (key[i]) sum += expf(value_of(key[i]) - most);
+      if (key[i]) sum += expf(K::value(key[i]) - most);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
   }
   float p[2] = {0.f, 0.f};   // slots lane and lane + 32
   int id[2] = {-1, -1};
   for (int j = 0; j < k; ++j) {
-    const uint32_t m = __reduce_max_sync(0xffffffffu, best);
+    const uint32_t m = j == 0 ? top : __reduce_max_sync(0xffffffffu, best);
     if (m == 0) break;
     const int mine = best == m ? lane + 32 * at : 0x7fffffff;
-    const int e = __reduce_min_sync(0xffffffffu, mine);
+    const int e = K::kIndexed ? K::index(m) : __reduce_min_sync(0xffffffffu, mine);
     if (mine == e) {
 #pragma unroll
       for (int i = 0; i < EPL; ++i)
@@ -81,7 +103,7 @@ __device__ __forceinline__ void topk_token(const T* __restrict__ logits, int E, 
       rescan();
     }
     if ((j & 31) == lane) {
-      p[j >> 5] = expf(value_of(m) - most);
+      p[j >> 5] = expf(K::value(m) - most);
       id[j >> 5] = e;
     }
   }
@@ -115,28 +137,32 @@ __global__ void __launch_bounds__(256) route_topk_kernel(const T* __restrict__ l
 
 // Stable counting sort of the pairs by expert, in one cluster (one CTA for small T), and the
 // top-k of the tokens before it when `topk` is set.  Every warp owns a run of consecutive
-// tokens and counts its pairs by expert in its own row of shared memory (lanes that hold the
-// same expert find each other with match_any, the lowest of them adds); the counts are
-// scanned over the warps of the CTA, over the CTAs through distributed shared memory, and
-// over the experts; a second walk over the pairs hands out the positions in order.  No
-// atomics, so the result does not depend on timing.
+// tokens, a lane a token at a time.  Counts: every lane adds its pairs to the warp's own row of
+// shared memory; the rows are scanned over the warps of the CTA, over the CTAs through
+// distributed shared memory, and over the experts.  Positions: a token has an expert once at
+// most, so the pairs of an expert among 32 tokens are a bit mask (OR-ed in shared memory), and
+// a pair's rank is the number of lower bits.  Integer additions and ORs only, so the result does
+// not depend on timing.  (Finding equal experts with match_any instead took 36 us at 131072
+// pairs.)
 template <typename T, int EPL>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(1024, 1)
     route_group_kernel(const T* __restrict__ logits, float* __restrict__ weights,
                        int* __restrict__ experts, int* __restrict__ offsets,
                        int* __restrict__ rows, int n, int E, int k, int renormalize, int topk,
                        int csize) {
   extern __shared__ int sh[];
-  int* hist = sh;               // [WARPS][E]
-  int* total = sh + WARPS * E;  // [E] this CTA's pairs
-  int* start = total + E;       // [E] first position of the expert, then of this CTA's pairs
+  const int nwarps = blockDim.x / 32;
+  int* hist = sh;                                                 // [nwarps][E]
+  uint32_t* mask = reinterpret_cast<uint32_t*>(sh + nwarps * E);  // [nwarps][E]
+  int* total = sh + 2 * nwarps * E;                               // [E] this CTA's pairs
+  int* start = total + E;                                         // [E] first position of the expert
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int cta = blockIdx.x;   // the grid is one cluster
   ptx::grid_launch_dependents();
-  for (int i = threadIdx.x; i < WARPS * E; i += THREADS) hist[i] = 0;
+  for (int i = threadIdx.x; i < 2 * nwarps * E; i += blockDim.x) sh[i] = 0;
   ptx::grid_dependency_wait();
-  const int per = (n + csize * WARPS - 1) / (csize * WARPS);
-  const long long first = (long long)(cta * WARPS + warp) * per;
+  const int per = (n + csize * nwarps - 1) / (csize * nwarps);
+  const long long first = (long long)(cta * nwarps + warp) * per;
   const int t0 = (int)(first < n ? first : n), t1 = (int)(first + per < n ? first + per : n);
   if (topk)
     for (int t = t0; t < t1; ++t)
@@ -144,25 +170,19 @@ __global__ void __launch_bounds__(THREADS, 1)
                          experts + (size_t)t * k, lane);
   __syncthreads();
   int* mine = hist + warp * E;
-  const long long i0 = (long long)t0 * k, i1 = (long long)t1 * k;
-  constexpr int U = 4;  // loads in flight a lane
-  for (long long i = i0; i < i1; i += 32 * U) {
-    int e[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      e[u] = i + 32 * u + lane < i1 ? experts[i + 32 * u + lane] : -1;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const uint32_t peers = __match_any_sync(0xffffffffu, e[u]);
-      if (e[u] >= 0 && lane == __ffs(peers) - 1) mine[e[u]] += __popc(peers);
-      __syncwarp();
+  uint32_t* bits = mask + warp * E;
+  for (int t = t0 + lane; t < t1; t += 32) {
+#pragma unroll 8
+    for (int j = 0; j < k; ++j) {
+      const int e = experts[(size_t)t * k + j];
+      if (e >= 0) atomicAdd(mine + e, 1);
     }
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < E; e += THREADS) {
+  for (int e = threadIdx.x; e < E; e += blockDim.x) {
     int run = 0;
 #pragma unroll 8
-    for (int w = 0; w < WARPS; ++w) {
+    for (int w = 0; w < nwarps; ++w) {
       const int c = hist[w * E + e];
       hist[w * E + e] = run;
       run += c;
@@ -171,8 +191,12 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
   if (csize > 1) ptx::cluster_sync_all(); else __syncthreads();
   // all pairs of each expert, and how many of them lie in earlier CTAs
-  for (int e = threadIdx.x; e < E; e += THREADS) {
-    int all = 0, before = 0;
+  int before[1024 / 256] = {};  // of experts threadIdx.x, + blockDim.x, ... (at least 256 threads)
+#pragma unroll
+  for (int i = 0; i < 1024 / 256; ++i) {
+    const int e = threadIdx.x + i * blockDim.x;
+    if (e >= E) break;
+    int all = 0;
     if (csize > 1) {
       const uint32_t here = ptx::smem_u32(total + e);
       for (int c = 0; c < csize; ++c) {
@@ -180,17 +204,16 @@ __global__ void __launch_bounds__(THREADS, 1)
         asm volatile("ld.shared::cluster.u32 %0, [%1];"
                      : "=r"(v) : "r"(ptx::map_to_rank(here, c)) : "memory");
         all += v;
-        if (c < cta) before += v;
+        if (c < cta) before[i] += v;
       }
     } else {
       all = total[e];
     }
     start[e] = all;
-    for (int w = 0; w < WARPS; ++w) hist[w * E + e] += before;
   }
   __syncthreads();
   if (warp == 0) {  // exclusive scan over the experts
-    const int chunk = (E + 31) / 32, e0 = lane * chunk, e1 = min(E, e0 + chunk);
+    const int chunk = (E + 31) / 32, e0 = min(E, lane * chunk), e1 = min(E, e0 + chunk);
     int sum = 0;
     for (int e = e0; e < e1; ++e) sum += start[e];
     int run = sum;
@@ -199,6 +222,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int o = __shfl_up_sync(0xffffffffu, run, off);
       if (lane >= off) run += o;
     }
+    if (cta == 0 && lane == 31) offsets[E] = run;
     run -= sum;
     for (int e = e0; e < e1; ++e) {
       const int c = start[e];
@@ -206,24 +230,34 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (cta == 0) offsets[e] = run;
       run += c;
     }
-    if (cta == 0 && e1 == E && e0 < E) offsets[E] = run;
   }
   __syncthreads();
-  for (long long i = i0; i < i1; i += 32 * U) {
-    int e[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      e[u] = i + 32 * u + lane < i1 ? experts[i + 32 * u + lane] : -1;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const uint32_t peers = __match_any_sync(0xffffffffu, e[u]);
-      int pos = -1;
-      if (e[u] >= 0) pos = start[e[u]] + mine[e[u]] + __popc(peers & ((1u << lane) - 1u));
-      __syncwarp();
-      if (e[u] >= 0 && lane == __ffs(peers) - 1) mine[e[u]] += __popc(peers);
-      __syncwarp();
-      if (i + 32 * u + lane < i1) rows[i + 32 * u + lane] = pos;
+  for (int i = 0; i < 1024 / 256; ++i) {
+    const int e = threadIdx.x + i * blockDim.x;
+    if (e < E) start[e] += before[i];
+  }
+  __syncthreads();
+  for (int b = t0; b < t1; b += 32) {  // warp-uniform
+    const int t = b + lane;
+    const bool in = t < t1;
+    for (int j = 0; in && j < k; ++j) {
+      const int e = experts[(size_t)t * k + j];
+      if (e >= 0) atomicOr(bits + e, 1u << lane);
     }
+    __syncwarp();
+    for (int j = 0; in && j < k; ++j) {
+      const int e = experts[(size_t)t * k + j];
+      rows[(size_t)t * k + j] =
+          e < 0 ? -1 : start[e] + mine[e] + __popc(bits[e] & ((1u << lane) - 1u));
+    }
+    __syncwarp();
+    if (b + 32 < t1)
+      for (int e = lane; e < E; e += 32) {
+        mine[e] += __popc(bits[e]);
+        bits[e] = 0u;
+      }
+    __syncwarp();
   }
   if (csize > 1) ptx::cluster_sync_all();  // no CTA leaves while another reads its totals
 }
@@ -394,13 +428,15 @@ __device__ __forceinline__ void store8(T* __restrict__ p, int left, const float 
 }
 
 // out[t] = sum_j w[t, j] y[rows[t, j]] (+ residual[t]): a thread per 8 columns of a token,
-// fp32 sums with j ascending, four rows' loads in flight.
-template <typename TI, typename TO, bool VEC>
+// fp32 sums with j ascending.  Bound by HBM: U rows' loads are in flight a thread, as loaded
+// (8 rows of bf16: 172 us at 8192 tokens of 8 rows x 4096 with 4 in flight and widened at once).
+template <typename TI, typename TO, bool VEC, int U>
 __global__ void __launch_bounds__(128) combine_kernel(const TI* __restrict__ y,
                                                       const int* __restrict__ rows,
                                                       const float* __restrict__ weights,
                                                       const TO* residual, TO* out, int T, int k,
                                                       int N, int R, int* err) {
+  constexpr int RAW = VEC ? (int)sizeof(TI) / 2 : 1;  // 16-byte words of 8 elements
   ptx::grid_launch_dependents();
   ptx::grid_dependency_wait();
   const int c = (blockIdx.x * 128 + threadIdx.x) * 8;
@@ -408,33 +444,58 @@ __global__ void __launch_bounds__(128) combine_kernel(const TI* __restrict__ y,
   const int left = N - c;
   for (int t = blockIdx.y; t < T; t += gridDim.y) {
     float acc[8] = {};
-    float res[8];
-    if (residual) load8<TO, VEC>(residual + (size_t)t * N + c, left, res);
-    constexpr int U = 4;
     for (int j0 = 0; j0 < k; j0 += U) {
-      float v[U][8], w[U];
+      uint4 raw[U][RAW];
+      float w[U];
+      int row[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        int r = j0 + u < k ? __ldg(rows + (size_t)t * k + j0 + u) : -1;
-        if (r >= R) {
-          if (c == 0) atomicCAS(err, 0, DEVERR_BAD_INDEX);
-          r = -1;
-        }
-        // a slot without a row adds nothing, whatever its weight
-        w[u] = r < 0 ? 0.f : weights ? __ldg(weights + (size_t)t * k + j0 + u) : 1.f;
-        if (r >= 0) {
-          load8<TI, VEC>(y + (size_t)r * N + c, left, v[u]);
-        } else {
+        row[u] = j0 + u < k ? __ldg(rows + (size_t)t * k + j0 + u) : -1;
+        w[u] = weights && j0 + u < k ? __ldg(weights + (size_t)t * k + j0 + u) : 1.f;
+      }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[u][i] = 0.f;
+      for (int u = 0; u < U; ++u) {
+        if (row[u] >= R) {
+          if (c == 0) atomicCAS(err, 0, DEVERR_BAD_INDEX);
+          row[u] = -1;
+        }
+        if constexpr (VEC) {
+#pragma unroll
+          for (int h = 0; h < RAW; ++h)
+            raw[u][h] = row[u] >= 0
+                ? __ldcs(reinterpret_cast<const uint4*>(y + (size_t)row[u] * N + c) + h)
+                : make_uint4(0u, 0u, 0u, 0u);
         }
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u) {
+        if (row[u] < 0) continue;  // a slot without a row adds nothing, whatever its weight
+        float v[8];
+        if constexpr (!VEC) {
+          load8<TI, false>(y + (size_t)row[u] * N + c, left, v);
+        } else if constexpr (sizeof(TI) == 2) {
+          const uint32_t q[4] = {raw[u][0].x, raw[u][0].y, raw[u][0].z, raw[u][0].w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] = __fmaf_rn(w[u], v[u][i], acc[i]);
+          for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(q[i] << 16);
+            v[2 * i + 1] = __uint_as_float(q[i] & 0xffff0000u);
+          }
+        } else {
+#pragma unroll
+          for (int h = 0; h < RAW; ++h) {
+            v[4 * h] = __uint_as_float(raw[u][h].x);
+            v[4 * h + 1] = __uint_as_float(raw[u][h].y);
+            v[4 * h + 2] = __uint_as_float(raw[u][h].z);
+            v[4 * h + 3] = __uint_as_float(raw[u][h].w);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] = __fmaf_rn(w[u], v[i], acc[i]);
+      }
     }
     if (residual) {
+      float res[8];
+      load8<TO, VEC>(residual + (size_t)t * N + c, left, res);
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc[i] += res[i];
     }
@@ -470,22 +531,23 @@ template <typename T, int EPL>
 qgemm_status route_t(qgemm_stream_s* s, const T* logits, float* weights, int* experts,
                      int* offsets, int* rows, int n, int E, int k, int renormalize) {
   // Top-k in the grouping kernel while its CTAs can hold the tokens a few to a warp; beyond
-  // that over the whole GPU first.
-  const int csize = n <= WARPS ? 1 : CLUSTER;
-  const bool fused = n <= 2 * WARPS * CLUSTER;
+  // that over the whole GPU first.  Two rows of E words a warp: 32 warps up to 512 experts.
+  const int warps = E <= 512 ? 32 : 16;
+  const int csize = n <= 32 ? 1 : CLUSTER;
+  const bool fused = n <= 2 * warps * CLUSTER;
   if (!fused) {
     const cudaError_t e = launch(route_topk_kernel<T, EPL>, dim3((n + 7) / 8), 256, 0, s->stream,
                                  1, logits, weights, experts, n, E, k, renormalize);
     if (e != cudaSuccess) return cuda_fail(e, "route_topk launch");
   }
-  const size_t smem = sizeof(int) * (size_t)(WARPS + 2) * E;
+  const size_t smem = sizeof(int) * (size_t)(2 * warps + 2) * E;
   const auto kern = route_group_kernel<T, EPL>;
   if (smem > 48 * 1024) {
     const cudaError_t e =
         cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(route_group)");
   }
-  return cuda_fail(launch(kern, dim3(csize), THREADS, smem, s->stream, csize, logits, weights,
+  return cuda_fail(launch(kern, dim3(csize), 32 * warps, smem, s->stream, csize, logits, weights,
                           experts, offsets, rows, n, E, k, renormalize, fused ? 1 : 0, csize),
                    "route_group launch");
 }
@@ -534,8 +596,13 @@ cudaError_t combine_t(qgemm_stream_s* s, const void* y, const int* rows, const f
   const TO* ri = static_cast<const TO*>(residual);
   TO* o = static_cast<TO*>(out);
   int* err = s->dev->d_err;
-  return vec ? launch(combine_kernel<TI, TO, true>, g, 128, 0, s->stream, 1, yi, rows, weights, ri, o, n, k, N, R, err)
-             : launch(combine_kernel<TI, TO, false>, g, 128, 0, s->stream, 1, yi, rows, weights, ri, o, n, k, N, R, err);
+  auto go = [&](auto kern) {
+    return launch(kern, g, 128, 0, s->stream, 1, yi, rows, weights, ri, o, n, k, N, R, err);
+  };
+  if (!vec) return go(combine_kernel<TI, TO, false, 2>);
+  if (k <= 2) return go(combine_kernel<TI, TO, true, 2>);
+  if (k <= 4) return go(combine_kernel<TI, TO, true, 4>);
+  return go(combine_kernel<TI, TO, true, 8>);
 }
 
 }  // namespace route

@@ -282,3 +282,15 @@ def test_combine_onto_the_residual_in_place(gpu):
     ops.combineRows(y, rows, w, x, T, k, N, T * k, residual=x)
     st.sync()
     assert torch.equal(x, apart)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_route_infinity_beats_the_largest_finite_value(gpu, dtype):
+    """+inf counts as the largest finite fp32: above bf16's largest, equal to fp32's own."""
+    big = 3.3895313892515355e38  # bf16's largest
+    v = np.zeros((70, 20))
+    v[:, 4] = big
+    v[:, 11] = np.inf
+    v[3, 11] = -np.inf
+    check_route(gpu, v, 3, True, dtype)
+    check_route(gpu, v, 3, False, dtype)

@@ -1262,8 +1262,8 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
     tok_max = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : cap;
     box = tok_max < 32 ? tok_max : 32;
   } else {  // equal blocks, each one box
-    const int nblk = (a.M + cap - 1) / cap;
-    tok_max = ((a.M + nblk - 1) / nblk + 15) / 16 * 16;
+    const int blocks = (a.M + cap - 1) / cap;
+    tok_max = ((a.M + blocks - 1) / blocks + 15) / 16 * 16;
     box = tok_max;
   }
   // K over c CTAs, and weight rows a tile, so that the rounds come out full.  A round takes the
@@ -1274,7 +1274,8 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
   // 14.7 with 1; 33 x 11008 x 4096 int8 gated: 21.2 us with c = 2 and 112 rows, 22.5 with c = 1
   // and 128).
   const int ksteps = (p.num_k_blocks + strm::STEP - 1) / strm::STEP;
-  const long long groups_tok = (long long)groups * ((avg + tok_max - 1) / tok_max);
+  const int nblk = (avg + tok_max - 1) / tok_max;
+  const long long groups_tok = (long long)groups * nblk;
   const double tok = avg < tok_max ? avg : tok_max;
   const double kb_us = (a.gated ? 0.22 : 0.17) + 0.0009 * tok;
   auto both = [](double x, double y) { return x > y ? x + 0.25 * y : y + 0.25 * x; };
@@ -1299,7 +1300,8 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
       double cta = (ksteps + c - 1) / c * strm::STEP * kb_us + 0.1;
       if (c > 1 && cta < 1.2 + 0.03 * tok) cta = 1.2 + 0.03 * tok;  // an exchange a tile
       const int ctas = c * ds->clusters[i];
-      const double tile_hbm = (double)r * a.K * es / (6.2e6 * (ctas < sms ? ctas : sms) / sms);
+      // (the token blocks of a group run side by side and share their weights in L2)
+      const double tile_hbm = (double)r * a.K * es / nblk / (6.2e6 * (ctas < sms ? ctas : sms) / sms);
       const double us = (r < WROWS ? 1.03 : 1.0) * (full * both(cta, ds->clusters[i] * tile_hbm) +
                         (rest ? both(cta, rest * tile_hbm) : 0.0)) + (c > 1 ? 0.6 + 0.05 * tok : 0.0);
       if (stream_us == 0 || us < stream_us) { stream_us = us; pick = i; rows = r; }
@@ -1318,10 +1320,10 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
   // (SEG costs the pair kernel half its time more: 142 us against 100 streaming for those rows)
   const double pair_us = 0.5 + (seg ? 1.5 : 1.0) * pfull * pair_round(pairs, pair_n) +
       (prest ? (seg ? 1.5 : 1.0) * pair_round(prest, pair_n / (pairs / prest < 4 ? pairs / prest : 4)) : 0.0);
-  // Which kernel: the model where a group has up to 96 rows (measured, bf16 4096 x 4096: 64 rows
-  // 12.2 us streaming, 19.5 in pairs; 128 rows 17.7 and 19.9; 256 rows 24.6 and 20.9; 11008 x
-  // 4096: 96 rows 22.6 and 24.8; 128 rows 34.9 and 25.6).
-  const bool use_pair = avg > 96 || pair_us < stream_us;
+  // Which kernel (measured, bf16 4096 x 4096: 64 rows 12.2 us streaming, 19.5 in pairs; 256 rows
+  // 19.6 and 20.6; 512 rows 32 and 25; 11008 x 4096: 96 rows 22.7 and 24.7; 128 rows 31.5 and
+  // 25.6).
+  const bool use_pair = pair_us < stream_us;
 
   cudaLaunchConfig_t cfg = {};
   cfg.stream = s->stream;

@@ -1213,7 +1213,8 @@ bool linear_tcgen05_supported(const qgemm_device_s* d, const LinArgs& a, const c
   if (!d->tcgen05) return no("device is not sm_100 (tcgen05 unavailable)");
   if (d->smem_optin < (size_t)lin::SMEM_MAX) return no("not enough shared memory per block");
   if (a.K <= 0) return no("K == 0");
-  // tiles and rows are counted in 32 bits
+  // tiles, rows and the bytes of a row are counted in 32 bits
+  if (a.K > (1 << 29)) return no("K > 2^29");
   if (a.M > (1 << 30) || ((long long)a.M / 16 + a.E) * (a.N / 64 + 1) > (1ll << 30))
     return no("more than 2^30 tiles");
   if (((long long)a.K * es) % 16 != 0) return no("K is not a multiple of 16 bytes");
@@ -1385,17 +1386,16 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
   }
   // weight boxes: all of a CTA's rows, or (gated) runs of 8 and the 5-D map over them
   CUtensorMap tmW, tmG, tmX;
-  memset(&tmG, 0, sizeof(tmG));
   if (!make_map(&tmW, a.w, (uint64_t)a.K * es, (uint64_t)a.E * p.ep.nw, (uint64_t)a.K * es,
                 a.gated ? 8 : p.rows))
     return fail(QGEMM_ERR_CUDA, "cuTensorMapEncodeTiled failed for the weights");
+  tmG = tmW;  // not used where no tile of the layer lies in whole blocks of 8 features
   if (a.gated && a.N / 8 >= p.rows / 16 &&
       !make_gated_map(&tmG, a.w, (uint64_t)a.K * es, a.N, a.E, p.rows / 16))
     return fail(QGEMM_ERR_CUDA, "cuTensorMapEncodeTiled failed for the gated weights");
   if (!make_map(&tmX, a.x, (uint64_t)a.K * es, (uint64_t)a.M, (uint64_t)a.ldx * es, box))
     return fail(QGEMM_ERR_CUDA, "cuTensorMapEncodeTiled failed for x");
-  CUtensorMap tmXs;
-  memset(&tmXs, 0, sizeof(tmXs));
+  CUtensorMap tmXs = tmX;  // the pair kernel's boxes for part tiles
   if (use_pair && !make_map(&tmXs, a.x, (uint64_t)a.K * es, (uint64_t)a.M, (uint64_t)a.ldx * es, pair::BOX))
     return fail(QGEMM_ERR_CUDA, "cuTensorMapEncodeTiled failed for x");
   return cuda_fail(cudaLaunchKernelEx(&cfg, kern, tmW, tmG, tmX, tmXs, p), "linear launch");

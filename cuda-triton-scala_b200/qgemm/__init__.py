@@ -9,13 +9,14 @@ from ._lib import (ACT_GELU, ACT_GELU_TANH, ACT_NONE, ACT_RELU, ACT_SILU, ALGO_A
                    ALGO_TCGEN05, B_KN, B_NK, BF16, F32, QGemmError, last_error, lib,
                    status_name)
 from .comm import NCCLCommunicator, OutputWindow
+from .experts import ExpertMLP
 from .ops import (BLASOps, CUDARuntimeJavaBridge, CutlassGemm, MatrixOps, QuantizedGemmOps,
                   TensorCoreOps, shard_columns)
 from .runtime import Buffer, Device, Stream, device_count
 
 __all__ = [
     "ACT_GELU", "ACT_GELU_TANH", "ACT_NONE", "ACT_RELU", "ACT_SILU", "ALGO_AUTO", "ALGO_SIMT", "ALGO_TCGEN05", "B_KN", "B_NK", "BF16", "F32", "QGemmError",
-    "last_error", "lib", "status_name", "BLASOps", "CUDARuntimeJavaBridge", "CutlassGemm",
+    "last_error", "lib", "status_name", "BLASOps", "CUDARuntimeJavaBridge", "CutlassGemm", "ExpertMLP",
     "MatrixOps", "QuantizedGemmOps", "TensorCoreOps", "shard_columns", "Buffer", "Device",
     "Stream", "device_count", "NCCLCommunicator", "OutputWindow",
 ]

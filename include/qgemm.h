@@ -417,7 +417,10 @@ QGEMM_API qgemm_status qgemm_gemv_f32(qgemm_stream_t s, uint64_t A, uint64_t x, 
  *             layer then adds onto the stream in place)
  *   out       [M, ldc] of out_dtype (QGEMM_BF16 or QGEMM_F32); nothing past column N of a
  *             row is written
- * Everything is fp32 up to one rounding (RNE) to out_dtype.  Deterministic: the same call
+ * Everything is fp32 up to one rounding (RNE) to out_dtype.  bf16 sums run on the tensor
+ * cores, whose fp32 additions truncate (about 1e-9 of the result a value of K, far below a
+ * bf16 step); for fp32 outputs they are taken in pieces of 512 values that are added rounding
+ * to nearest (about 5e-7, whatever K).  Deterministic: the same call
  * gives the same bits, whatever ran before.  Nothing is allocated and no scratch is used,
  * so calls on different streams, and captured graphs, are independent.  QGEMM_ALGO_AUTO
  * runs on the tensor cores when K is a multiple of 16 bytes and x, w and their rows are

@@ -33,10 +33,23 @@ struct Epi {
 // a bf16 step: the full-precision ones made the gated layer at 8192 x 28672 x 4096 int8 28 %
 // slower than the same layer without an activation.  __fdividef gives 0 where 1 + exp(-v)
 // passes 2^126, which is the limit there.
+// GELU is max(v, 0) - 0.5 |v| erfc(|v| / sqrt 2), erfc(x) = exp(-x^2) P(1 / (1 + p x)) with the
+// degree-5 P of Abramowitz and Stegun 7.1.26 (absolute error 1.5e-7, and no cancellation for
+// negative v, where 1 + erf loses the small result); about half of erff's instructions, which
+// the last tile's epilogue exposes.
+__device__ __forceinline__ float gelu(float v) {
+  const float a = fminf(fabsf(v), 30.f);  // exp(-a^2 / 2) is 0 from 15 on
+  const float t = __fdividef(1.f, fmaf(0.3275911f * 0.70710678118654752f, a, 1.f));
+  const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f),
+                                   -0.284496736f), 0.254829592f);
+  const float y = fmaxf(v, 0.f) - 0.5f * a * p * __expf(-0.5f * a * a);
+  return v != v ? v : y;
+}
+
 __device__ __forceinline__ float activate(int act, float v) {
   switch (act) {
     case QGEMM_ACT_RELU: return v > 0.f ? v : (v != v ? v : 0.f);
-    case QGEMM_ACT_GELU: return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
+    case QGEMM_ACT_GELU: return gelu(v);
     case QGEMM_ACT_GELU_TANH: {  // 0.5 v (1 + tanh u) = v / (1 + exp(-2 u))
       const float u = 0.79788456080286536f * (v + 0.044715f * v * v * v);
       return __fdividef(v, 1.f + __expf(-2.f * u));

@@ -6,21 +6,23 @@
 //
 // Both kernels compute the transposed tile: the weights are the MMA's A operand (M = 128
 // weight rows a CTA) and the tokens its B operand.  The tokens then lie along the MMA's N,
-// which is a run-time field of the instruction descriptor: a group of 44 rows costs MMAs of
-// 48 (or 64) columns instead of a whole 128- or 256-row tile, and one token costs a 16-column
+// which is a run-time field of the instruction descriptor: a group of 44 rows costs MMAs of 48
+// (or 64) columns instead of a whole 128- or 256-row tile, and one token costs a 16-column
 // one.  An accumulator column is a token, a TMEM lane a feature: bias and weight scale are
-// per-lane constants, and a staging buffer [token][128 features] in shared memory turns the
-// tile so that a warp stores one token's 128 features as one contiguous run.  Gated layers
-// give each CTA 64 gate rows and the 64 up rows of the same features, so both halves of a
-// product meet in the staging buffer.
+// per-lane constants.  Gated layers lay 8 gate rows and the 8 up rows of the same features by
+// turns, so both halves of a product meet in one warp.
 //
 //   linear_pair_kernel    many rows: CTA pairs (tcgen05 cta_group::2), tiles of 256 weight
 //       rows x up to 256 tokens, persistent, two accumulators so that the epilogue of a tile
-//       overlaps the next tile's MMAs.  Bound by the tensor pipe.
-//   linear_stream_kernel  few rows: one CTA per tile of 128 weight rows x up to 128 tokens,
-//       persistent; a cluster of 1, 2, 4 or 8 CTAs cuts K and joins its partial sums through
-//       distributed shared memory in rank order (so no scratch, no atomics, the same bits
-//       every time).  Bound by reading the weights once.
+//       overlaps the next tile's MMAs.  Bound by the tensor pipe and, under sustained load, by
+//       the power cap: int8 gated 8192 x 28672 x 4096 0.68 ms (2.83 POPS), bf16 4096 x 4096 x
+//       11008 with bias, gelu and residual 265 to 280 us (1.32 to 1.39 PFLOP/s).
+//   linear_stream_kernel  few rows: one CTA per tile of up to 128 weight rows x up to 96
+//       tokens, two k-blocks a stage, persistent; a cluster of 1, 2, 4 or 8 CTAs cuts K and
+//       joins its partial sums through distributed shared memory in rank order (so no scratch,
+//       no atomics, the same bits every time).  Bound by reading the weights once: 940 MB of
+//       experts' weights in 143 us (6.6 TB/s); small layers by 3.4 us of launch, first copy and
+//       exchange (1 x 4096 x 4096 bf16: 8.9 us).
 //
 // Experts: offsets[E + 1] are read on the device; every CTA lists the experts' tiles in
 // shared memory (prefix sums) and walks the same persistent schedule, so the host never
@@ -668,6 +670,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
       const Lane<GATED> f =
           lane_of<KIND, GATED>(p.ep, it_.e, (it_.wb * 2 + (int)rank) * p.feats, WROWS, q, lane);
       const int chunks = (it_.n + CHUNK - 1) / CHUNK;
+      // this warp's part of the residual into L2 while the MMAs run: its loads come chunk by
+      // chunk, and the last tile's epilogue waits for every one
+      if (p.ep.residual) {
+        const int os = p.ep.out_f32 ? 4 : 2;
+        const int f0 = (it_.wb * 2 + (int)rank) * p.feats + q * (GATED ? 16 : 32);
+        const char* at = static_cast<const char*>(p.ep.residual) + ((size_t)it_.t0 * p.ep.ldr + f0) * os;
+        for (int t = grp * 32 + lane; t < it_.n && f0 < p.ep.N; t += 64)
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(at + (size_t)t * p.ep.ldr * os));
+      }
       // Waits for accumulator it & 1; a warp whose wait ran out stores nothing.
       auto acc_ready = [&]() {
         bool ok = ptx::mbar_wait(tfull_bar(it & 1), (uint32_t)((it >> 1) & 1), abort_flag, p.wait_ns);

@@ -171,13 +171,19 @@ __global__ void __launch_bounds__(1024, 1)
   __syncthreads();
   int* mine = hist + warp * E;
   uint32_t* bits = mask + warp * E;
-  for (int t = t0 + lane; t < t1; t += 32) {
-#pragma unroll 8
-    for (int j = 0; j < k; ++j) {
-      const int e = experts[(size_t)t * k + j];
-      if (e >= 0) atomicAdd(mine + e, 1);
+  // calls fn(slot, expert) for a token's chosen experts, eight slots' loads in flight
+  auto each_pair = [&](int t, auto&& fn) {
+    for (int j0 = 0; j0 < k; j0 += 8) {
+      int ex[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ex[j] = j0 + j < k ? experts[(size_t)t * k + j0 + j] : -2;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (ex[j] > -2) fn(j0 + j, ex[j]);
     }
-  }
+  };
+  for (int t = t0 + lane; t < t1; t += 32)
+    each_pair(t, [&](int, int e) { if (e >= 0) atomicAdd(mine + e, 1); });
   __syncthreads();
   for (int e = threadIdx.x; e < E; e += blockDim.x) {
     int run = 0;
@@ -241,16 +247,13 @@ __global__ void __launch_bounds__(1024, 1)
   for (int b = t0; b < t1; b += 32) {  // warp-uniform
     const int t = b + lane;
     const bool in = t < t1;
-    for (int j = 0; in && j < k; ++j) {
-      const int e = experts[(size_t)t * k + j];
-      if (e >= 0) atomicOr(bits + e, 1u << lane);
-    }
+    if (in) each_pair(t, [&](int, int e) { if (e >= 0) atomicOr(bits + e, 1u << lane); });
     __syncwarp();
-    for (int j = 0; in && j < k; ++j) {
-      const int e = experts[(size_t)t * k + j];
-      rows[(size_t)t * k + j] =
-          e < 0 ? -1 : start[e] + mine[e] + __popc(bits[e] & ((1u << lane) - 1u));
-    }
+    if (in)
+      each_pair(t, [&](int j, int e) {
+        rows[(size_t)t * k + j] =
+            e < 0 ? -1 : start[e] + mine[e] + __popc(bits[e] & ((1u << lane) - 1u));
+      });
     __syncwarp();
     if (b + 32 < t1)
       for (int e = lane; e < E; e += 32) {

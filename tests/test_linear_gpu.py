@@ -479,3 +479,33 @@ def test_linear_fp32_sums_keep_their_precision(gpu, M):
     assert (d <= bound).all()
     # and in the mean far below what one accumulator over all of K loses (9e-6 of the result)
     assert float(d.norm() / exact.norm()) < 2e-6
+
+
+@pytest.mark.parametrize("kind", ["bf16", "w8a8"])
+@pytest.mark.parametrize("M,K,out", [(6, 4096, "bf16"), (2000, 512, "bf16"), (2000, 2048, "f32")])
+def test_expert_linear_every_expert_empty(gpu, kind, M, K, out):
+    """No tile at all, in each kernel: nothing is written and nothing waits."""
+    run(gpu, Case(kind, M, 264, K, offsets=[0, 0, 0], out=out))
+    run(gpu, Case(kind, M, 264, K, offsets=[M, M, M], out=out))
+
+
+def test_linear_sizes_drawn(gpu):
+    """Sizes drawn over their logarithm, with every epilogue: the kernels and cuts that the
+    time model picks between."""
+    rng = np.random.default_rng(2024)
+
+    def log(lo, hi):
+        return int(round(np.exp(rng.uniform(np.log(lo), np.log(hi)))))
+
+    for i in range(120):
+        kind = "bf16" if rng.random() < 0.5 else "w8a8"
+        M, N, K = log(1, 900), log(8, 3000), log(1, 150) * 16
+        off = None
+        if rng.random() < 0.4:
+            E = int(rng.choice([1, 2, 7, 40]))
+            cuts = np.sort(rng.integers(0, M + 1, E + 1))
+            off = cuts.tolist()
+        run(gpu, Case(kind, M, N, K, act=ACTS[i % 5], gated=bool(rng.random() < 0.5),
+                      bias=bool(rng.random() < 0.5), residual=off is None and bool(rng.random() < 0.5),
+                      out="f32" if rng.random() < 0.4 else "bf16", offsets=off, seed=i),
+            qgemm.ALGO_TCGEN05)

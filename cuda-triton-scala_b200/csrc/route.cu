@@ -89,7 +89,7 @@ __device__ __forceinline__ void topk_token(const T* __restrict__ logits, int E, 
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
   }
-  float p[2] = {0.f, 0.f};   // slots lane and lane + 32
+  uint32_t won[2] = {0u, 0u};  // keys of slots lane and lane + 32
   int id[2] = {-1, -1};
   for (int j = 0; j < k; ++j) {
     const uint32_t m = j == 0 ? top : __reduce_max_sync(0xffffffffu, best);
@@ -103,10 +103,13 @@ __device__ __forceinline__ void topk_token(const T* __restrict__ logits, int E, 
       rescan();
     }
     if ((j & 31) == lane) {
-      p[j >> 5] = expf(K::value(m) - most);
+      won[j >> 5] = m;
       id[j >> 5] = e;
     }
   }
+  float p[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) p[h] = won[h] ? expf(K::value(won[h]) - most) : 0.f;
   if (renormalize) {
     sum = p[0] + p[1];
 #pragma unroll

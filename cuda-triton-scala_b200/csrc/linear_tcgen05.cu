@@ -738,7 +738,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
 // ---- the streaming kernel ------------------------------------------------------------------
 namespace strm {  // tiles of 16 to 96 tokens at most (Params::tok_max, a multiple of 16)
 constexpr int THREADS = 192;   // producer, MMA issuer, four epilogue warps
-constexpr int SEG_TOK = 64;    // tokens of a tile at most with SEG: three times as many columns
+constexpr int TOK = 96;        // tokens of a tile at most: more leave too few stages
 constexpr int XTOK = 64;       // tokens of an exchange at most (SPLIT)
 constexpr int STEP = 2;        // k-blocks of a stage: one barrier round for both
 }  // namespace strm
@@ -1159,7 +1159,7 @@ static const Kern kStream[3][2][2] = {
     {{linear_stream_kernel<KIND_BF16, false, true, false>, linear_stream_kernel<KIND_BF16, false, true, true>},
      {linear_stream_kernel<KIND_BF16, true, true, false>, linear_stream_kernel<KIND_BF16, true, true, true>}}};
 
-static_assert(pair::SEG_TOK <= 128 && 3 * strm::SEG_TOK <= 256, "TMEM columns of SEG");
+static_assert(pair::SEG_TOK <= 128 && 3 * strm::TOK <= 512, "TMEM columns of SEG");
 
 // The tensor cores add each MMA's products to the fp32 accumulator by truncation, so a sum
 // over K shrinks by about 9e-10 of itself a value of K (measured: 2.1e-6 at K = 2048, 1.2e-5 at
@@ -1266,7 +1266,7 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
   const bool seg = a.kind == KIND_BF16 && a.out_dtype == QGEMM_F32 && p.num_k_blocks > SEG_KB;
   const int variant = a.kind == KIND_I8 ? 0 : seg ? 2 : 1;
   // ---- the streaming kernel's cut of the work ----
-  const int cap = seg ? strm::SEG_TOK : 96;  // 96: more tokens leave too few stages
+  const int cap = strm::TOK;
   int tok_max, box;
   if (a.offsets) {
     // tokens of a tile: twice the even share, so that a moderate skew stays in one tile
@@ -1292,7 +1292,7 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
   const double kb_us = (a.gated ? 0.22 : 0.17) + 0.0009 * tok;
   auto both = [](double x, double y) { return x > y ? x + 0.25 * y : y + 0.25 * x; };
   // a stage holds tok_max token rows and is filled in whole boxes
-  if (tok_max % box != 0 || tok_max > 96 || box > 128)
+  if (tok_max % box != 0 || tok_max > strm::TOK || box > 128)
     return fail(QGEMM_ERR_UNSUPPORTED, "token tile %d in boxes of %d", tok_max, box);
   double stream_us = 0;
   int pick = 0, rows = WROWS;
@@ -1367,7 +1367,7 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
     p.tok_max = tok_max;
     p.box = box;
     const int cols = (seg ? 3 : 2) * tok_max;  // accumulators, running sums
-    p.tmem_cols = cols <= 32 ? 32 : cols <= 64 ? 64 : cols <= 128 ? 128 : 256;
+    p.tmem_cols = cols <= 32 ? 32 : cols <= 64 ? 64 : cols <= 128 ? 128 : cols <= 256 ? 256 : 512;
     p.tok_round = 16;
     p.band = 1 << 20;  // token blocks run fastest: neighbours share the weights
     p.csize = 1 << pick;

@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include <cfloat>
+#include <mutex>
 
 #include "internal.h"
 #include "ptx.cuh"
@@ -533,6 +534,29 @@ cudaError_t launch(void (*kern)(P...), dim3 grid, int threads, size_t smem, cuda
   return cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
 }
 
+// The grouping kernel's shared memory at most: 16 warps' rows of 1024 experts.
+constexpr int GROUP_SMEM_MAX = (int)sizeof(int) * (2 * 16 + 2) * kMaxExperts;
+static_assert(GROUP_SMEM_MAX >= (int)sizeof(int) * (2 * 32 + 2) * 512, "32 warps up to 512 experts");
+
+// Opts a grouping kernel in to that size, once a device.  The permission belongs to the kernel,
+// not to a launch: set to each call's own need, one thread's call could lower it between another
+// thread's setting and its launch, which was then refused.
+template <typename T, int EPL>
+qgemm_status group_smem_opt_in(qgemm_stream_s* s) {
+  static std::mutex mu;
+  static bool done[64] = {};
+  const int ord = s->dev->ordinal;
+  if (ord < 0 || ord >= 64) return fail(QGEMM_ERR_UNSUPPORTED, "device ordinal %d >= 64", ord);
+  std::lock_guard<std::mutex> lock(mu);
+  if (!done[ord]) {
+    const cudaError_t e = cudaFuncSetAttribute(
+        route_group_kernel<T, EPL>, cudaFuncAttributeMaxDynamicSharedMemorySize, GROUP_SMEM_MAX);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(route_group)");
+    done[ord] = true;
+  }
+  return QGEMM_OK;
+}
+
 template <typename T, int EPL>
 qgemm_status route_t(qgemm_stream_s* s, const T* logits, float* weights, int* experts,
                      int* offsets, int* rows, int n, int E, int k, int renormalize) {
@@ -551,9 +575,8 @@ qgemm_status route_t(qgemm_stream_s* s, const T* logits, float* weights, int* ex
   const size_t smem = sizeof(int) * (size_t)(2 * warps + 2) * E;
   const auto kern = route_group_kernel<T, EPL>;
   if (smem > 48 * 1024) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(route_group)");
+    const qgemm_status st = group_smem_opt_in<T, EPL>(s);
+    if (st != QGEMM_OK) return st;
   }
   return cuda_fail(launch(kern, dim3(csize), 32 * warps, smem, s->stream, csize, logits, weights,
                           experts, offsets, rows, n, E, k, renormalize, fused ? 1 : 0, csize),

@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(256) linear_simt_kernel(const LinArgs a, Epi e
     const float s = ep.sx ? ep.sx[row] : 1.f;
     float z = dequant<KIND>(El::word(g[i]), swg, s);
     if (ep.bias) z = __fadd_rn(z, bg);
-    float v = activate(ep.act, z);
+    float v = ep.out_f32 ? activate<true>(ep.act, z) : activate<false>(ep.act, z);
     if (GATED) {
       float zu = dequant<KIND>(El::word(u[i]), swu, s);
       if (ep.bias) zu = __fadd_rn(zu, bu);

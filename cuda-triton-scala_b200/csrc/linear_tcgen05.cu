@@ -210,11 +210,12 @@ __device__ __forceinline__ void load_feat(const Epi& ep, int e, int n, Feat<GATE
 }
 
 // The residual of four features of a row, fetched before the products are needed.
+template <bool F32>
 __device__ __forceinline__ void load_residual(const Epi& ep, int row, int n, float (&r)[4]) {
   if (!ep.residual) return;
   const size_t at = (size_t)row * ep.ldr + n;
   if (ep.vec && n + 4 <= ep.N) {
-    if (ep.out_f32) {
+    if constexpr (F32) {
       const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(ep.residual) + at);
       r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w;
     } else {
@@ -228,19 +229,19 @@ __device__ __forceinline__ void load_residual(const Epi& ep, int row, int n, flo
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      r[i] = n + i < ep.N ? load_out(ep.residual, ep.out_f32, at + i) : 0.f;
+      r[i] = n + i < ep.N ? load_out(ep.residual, F32, at + i) : 0.f;
   }
 }
 
 // ACT is a compile-time choice: the switch sits outside the loops.
-template <int KIND, bool GATED, int ACT>
+template <int KIND, bool GATED, bool F32, int ACT>
 __device__ __forceinline__ void finish4(const Epi& ep, const Feat<GATED>& f, int row, float sx,
                                         const uint32_t (&g)[4], const uint32_t (&u)[4],
                                         const float (&res)[4]) {
   float v[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    v[i] = activate(ACT, __fadd_rn(dequant<KIND>(g[i], f.sg[i], sx), f.bg[i]));
+    v[i] = activate<F32>(ACT, __fadd_rn(dequant<KIND>(g[i], f.sg[i], sx), f.bg[i]));
     if constexpr (GATED)
       v[i] = __fmul_rn(v[i], __fadd_rn(dequant<KIND>(u[i], f.su[i], sx), f.bu[i]));
   }
@@ -250,7 +251,7 @@ __device__ __forceinline__ void finish4(const Epi& ep, const Feat<GATED>& f, int
   }
   const size_t at = (size_t)row * ep.ldc + f.n;
   if (ep.vec && f.n + 4 <= ep.N) {
-    if (ep.out_f32) {
+    if constexpr (F32) {
       *reinterpret_cast<float4*>(static_cast<float*>(ep.out) + at) =
           make_float4(v[0], v[1], v[2], v[3]);
     } else {
@@ -262,7 +263,7 @@ __device__ __forceinline__ void finish4(const Epi& ep, const Feat<GATED>& f, int
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (f.n + i < ep.N) store_out(ep.out, ep.out_f32, at + i, v[i]);
+      if (f.n + i < ep.N) store_out(ep.out, F32, at + i, v[i]);
   }
 }
 
@@ -298,14 +299,14 @@ __device__ __forceinline__ Lane<GATED> lane_of(const Epi& ep, int e, int f0, int
 // through a staging buffer in shared memory (256-byte runs of a token) the int8 layer at
 // 8192 x 28672 x 4096 took 827 us instead of 790.
 // FULL: all 16 tokens and all of the warp's features exist.
-template <int KIND, bool GATED, int ACT, bool FULL, typename Ready>
+template <int KIND, bool GATED, bool F32, int ACT, bool FULL, typename Ready>
 __device__ __forceinline__ void finish_chunk_t(const Epi& ep, const Lane<GATED>& l, int row0, int n,
                                                int lane, const uint32_t (&r)[16], Ready&& ready) {
   constexpr int NV = GATED ? 8 : 16;       // values a lane finishes
   const int hi = GATED ? lane / 8 % 2 : 0; // value i is token (GATED ? 2 i + hi : i)
   const int fe = l.f & ~1;                 // packed: features fe, fe + 1
   const int odd = l.f & 1;
-  const bool packed = !ep.out_f32 && ep.vec2;
+  const bool packed = !F32 && ep.vec2;
   // packed: pair i of this lane is token `first` + `step` i, feature fe
   const int first = GATED ? 2 * odd + hi : odd;
   constexpr int step = GATED ? 4 : 2;
@@ -330,7 +331,7 @@ __device__ __forceinline__ void finish_chunk_t(const Epi& ep, const Lane<GATED>&
       for (int i = 0; i < NV; ++i) {
         const int t = GATED ? 2 * i + hi : i;
         res[i] = FULL || (t < n && l.f < ep.N)
-                     ? load_out(ep.residual, ep.out_f32, (size_t)(row0 + t) * ep.ldr + l.f) : 0.f;
+                     ? load_out(ep.residual, F32, (size_t)(row0 + t) * ep.ldr + l.f) : 0.f;
       }
     }
   }
@@ -340,14 +341,14 @@ __device__ __forceinline__ void finish_chunk_t(const Epi& ep, const Lane<GATED>&
   for (int j = 0; j < 16; ++j) {
     const float s = KIND == KIND_I8 ? __shfl_sync(0xffffffffu, sx, j) : 0.f;
     v[j] = __fadd_rn(dequant<KIND>(r[j], l.sw, s), l.b);
-    if (!GATED) v[j] = activate(ACT, v[j]);
+    if (!GATED) v[j] = activate<F32>(ACT, v[j]);
   }
   if constexpr (GATED) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float other = __shfl_xor_sync(0xffffffffu, hi ? v[2 * i] : v[2 * i + 1], 8);
       const float gate = hi ? other : v[2 * i], up = hi ? v[2 * i + 1] : other;
-      v[i] = __fmul_rn(activate(ACT, gate), up);
+      v[i] = __fmul_rn(activate<F32>(ACT, gate), up);
     }
   }
   if (packed) {
@@ -376,19 +377,19 @@ __device__ __forceinline__ void finish_chunk_t(const Epi& ep, const Lane<GATED>&
       const int t = GATED ? 2 * i + hi : i;
       if (FULL || (t < n && l.f < ep.N)) {
         const float y = ep.residual ? __fadd_rn(v[i], res[i]) : v[i];
-        store_out(ep.out, ep.out_f32, (size_t)(row0 + t) * ep.ldc + l.f, y);
+        store_out(ep.out, F32, (size_t)(row0 + t) * ep.ldc + l.f, y);
       }
     }
   }
 }
 
-template <int KIND, bool GATED, int ACT, typename Ready>
+template <int KIND, bool GATED, bool F32, int ACT, typename Ready>
 __device__ __forceinline__ void finish_chunk(const Epi& ep, const Lane<GATED>& l, int row0, int n,
                                              int lane, const uint32_t (&r)[16], Ready&& ready) {
   if (n >= 16 && __all_sync(0xffffffffu, l.f < ep.N))
-    finish_chunk_t<KIND, GATED, ACT, true>(ep, l, row0, n, lane, r, ready);
+    finish_chunk_t<KIND, GATED, F32, ACT, true>(ep, l, row0, n, lane, r, ready);
   else
-    finish_chunk_t<KIND, GATED, ACT, false>(ep, l, row0, n, lane, r, ready);
+    finish_chunk_t<KIND, GATED, F32, ACT, false>(ep, l, row0, n, lane, r, ready);
 }
 
 // SEG: r (16 fp32 accumulator columns being loaded) plus the running sums at TMEM address
@@ -477,7 +478,8 @@ __device__ __forceinline__ bool pair_item(const Params& p, const Table& tb, int 
   return true;
 }
 
-template <int KIND, bool GATED, bool SEG>
+// F32: the output's type (and the residual's), and with it the form of the activation.
+template <int KIND, bool GATED, bool SEG, bool F32>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
     linear_pair_kernel(const __grid_constant__ CUtensorMap tmW,
                        const __grid_constant__ CUtensorMap tmG,
@@ -673,7 +675,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
       // this warp's part of the residual into L2 while the MMAs run: its loads come chunk by
       // chunk, and the last tile's epilogue waits for every one
       if (p.ep.residual) {
-        const int os = p.ep.out_f32 ? 4 : 2;
+        const int os = F32 ? 4 : 2;
         const int f0 = (it_.wb * 2 + (int)rank) * p.feats + q * (GATED ? 16 : 32);
         const char* at = static_cast<const char*>(p.ep.residual) + ((size_t)it_.t0 * p.ep.ldr + f0) * os;
         for (int t = grp * 32 + lane; t < it_.n && f0 < p.ep.N; t += 64)
@@ -714,7 +716,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
               uint32_t r[16];
               ptx::tmem_ld_32x32b_x16(acc + (uint32_t)(c * CHUNK), r);
               if (SEG) add_running(tmem_q + (uint32_t)(128 + c * CHUNK), kb > 0, r);
-              finish_chunk<KIND, GATED, decltype(act)::value>(
+              finish_chunk<KIND, GATED, F32, decltype(act)::value>(
                   p.ep, f, it_.t0 + c * CHUNK, it_.n - c * CHUNK, lane, r,
                   [] { if (!SEG) ptx::tmem_wait_ld(); });
             }
@@ -748,7 +750,7 @@ constexpr int STEP = 2;        // k-blocks of a stage: one barrier round for bot
 // ([token][32]) and sends every rank its run of tokens as one bulk copy, counted in bytes on the
 // receiver's barrier (word by word with st.async, 33 tokens took 2700 cycles a tile and 128
 // took 8500; DSMEM moves wide runs far better).  Otherwise a CTA finishes its own accumulator.
-template <int KIND, bool GATED, bool SEG, bool SPLIT>
+template <int KIND, bool GATED, bool SEG, bool F32, bool SPLIT>
 __global__ void __launch_bounds__(strm::THREADS, 1)
     linear_stream_kernel(const __grid_constant__ CUtensorMap tmW,
                          const __grid_constant__ CUtensorMap tmG,
@@ -1011,14 +1013,14 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
             const float sx = __shfl_sync(0xffffffffu, sxl, l & 31);
             if (l >= mine || ff.n >= ep.N) continue;
             float res[4];
-            load_residual(ep, row0 + l, ff.n, res);
+            load_residual<F32>(ep, row0 + l, ff.n, res);
             uint32_t g[4] = {0u, 0u, 0u, 0u}, u[4] = {0u, 0u, 0u, 0u};
             for (int c = 0; c < C; ++c) {
               const uint32_t at = recv + (uint32_t)(((c * 4 + fq) * slot + l) * 32 + fw) * 4u;
               add_words<KIND>(g, ld_shared_v4(at));
               if (GATED) add_words<KIND>(u, ld_shared_v4(at + 8 * 4));
             }
-            finish4<KIND, GATED, decltype(act)::value>(ep, ff, row0 + l, sx, g, u, res);
+            finish4<KIND, GATED, F32, decltype(act)::value>(ep, ff, row0 + l, sx, g, u, res);
           }
         });
         __syncwarp();
@@ -1038,7 +1040,7 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
       auto emit = [&](int c, const uint32_t (&r)[16]) {
         if constexpr (!SPLIT) {
           with_act(ep.act, [&](auto act) {
-            finish_chunk<KIND, GATED, decltype(act)::value>(ep, fl, t.t0 + c, t.n - c, lane, r, [] {});
+            finish_chunk<KIND, GATED, F32, decltype(act)::value>(ep, fl, t.t0 + c, t.n - c, lane, r, [] {});
           });
         } else {
           const int x0 = c / XT * XT;
@@ -1146,18 +1148,20 @@ static bool make_gated_map(CUtensorMap* m, const void* ptr, uint64_t width, int 
 
 using Kern = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const CUtensorMap,
                       const Params);
-// [int8, bf16, bf16 in segments][gated], the stream kernels also [K split]
-static const Kern kPair[3][2] = {
-    {linear_pair_kernel<KIND_I8, false, false>, linear_pair_kernel<KIND_I8, true, false>},
-    {linear_pair_kernel<KIND_BF16, false, false>, linear_pair_kernel<KIND_BF16, true, false>},
-    {linear_pair_kernel<KIND_BF16, false, true>, linear_pair_kernel<KIND_BF16, true, true>}};
-static const Kern kStream[3][2][2] = {
-    {{linear_stream_kernel<KIND_I8, false, false, false>, linear_stream_kernel<KIND_I8, false, false, true>},
-     {linear_stream_kernel<KIND_I8, true, false, false>, linear_stream_kernel<KIND_I8, true, false, true>}},
-    {{linear_stream_kernel<KIND_BF16, false, false, false>, linear_stream_kernel<KIND_BF16, false, false, true>},
-     {linear_stream_kernel<KIND_BF16, true, false, false>, linear_stream_kernel<KIND_BF16, true, false, true>}},
-    {{linear_stream_kernel<KIND_BF16, false, true, false>, linear_stream_kernel<KIND_BF16, false, true, true>},
-     {linear_stream_kernel<KIND_BF16, true, true, false>, linear_stream_kernel<KIND_BF16, true, true, true>}}};
+// The kernels of an operand kind, summed in segments or not, for one output type.
+struct Kerns {
+  Kern pair[2], stream[2][2];  // [gated], [gated][K split]
+};
+template <int KIND, bool SEG, bool F32>
+static constexpr Kerns kerns_of() {
+  return {{linear_pair_kernel<KIND, false, SEG, F32>, linear_pair_kernel<KIND, true, SEG, F32>},
+          {{linear_stream_kernel<KIND, false, SEG, F32, false>, linear_stream_kernel<KIND, false, SEG, F32, true>},
+           {linear_stream_kernel<KIND, true, SEG, F32, false>, linear_stream_kernel<KIND, true, SEG, F32, true>}}};
+}
+static const Kerns kInt8[2] = {kerns_of<KIND_I8, false, false>(), kerns_of<KIND_I8, false, true>()};
+static const Kerns kBf16[2] = {kerns_of<KIND_BF16, false, false>(), kerns_of<KIND_BF16, false, true>()};
+static const Kerns kBf16Seg = kerns_of<KIND_BF16, true, true>();
+static const Kerns* const kAll[] = {&kInt8[0], &kInt8[1], &kBf16[0], &kBf16[1], &kBf16Seg};
 
 static_assert(pair::SEG_TOK <= 128 && 3 * strm::TOK <= 512, "TMEM columns of SEG");
 
@@ -1185,11 +1189,11 @@ static qgemm_status device_setup(qgemm_stream_s* s, const DeviceSetup** out) {
   std::lock_guard<std::mutex> lock(mu);
   DeviceSetup& d = setup[ord];
   if (!d.ready) {
-    for (int k = 0; k < 3; ++k)
+    for (const Kerns* k : kAll)
       for (int g = 0; g < 2; ++g) {
-        cudaError_t e = cudaFuncSetAttribute(kPair[k][g], cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
+        cudaError_t e = cudaFuncSetAttribute(k->pair[g], cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
         for (int sp = 0; sp < 2 && e == cudaSuccess; ++sp)
-          e = cudaFuncSetAttribute(kStream[k][g][sp], cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
+          e = cudaFuncSetAttribute(k->stream[g][sp], cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
         if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(linear)");
       }
     for (int i = 0; i < 4; ++i) {
@@ -1206,7 +1210,7 @@ static qgemm_status device_setup(qgemm_stream_s* s, const DeviceSetup** out) {
       cfg.attrs = attr;
       cfg.numAttrs = 1;
       int n = 0;
-      const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kStream[0][0][1], &cfg);
+      const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kInt8[0].stream[0][1], &cfg);
       if (e != cudaSuccess) return cuda_fail(e, "cudaOccupancyMaxActiveClusters(linear)");
       d.clusters[i] = n;
     }
@@ -1246,7 +1250,6 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
   p.ep.sx = a.sx; p.ep.sw = a.sw; p.ep.bias = a.bias; p.ep.residual = a.residual;
   p.ep.out = a.out; p.ep.ldr = a.ldr; p.ep.ldc = a.ldc;
   p.ep.N = a.N; p.ep.nw = a.gated ? 2 * a.N : a.N;
-  p.ep.out_f32 = a.out_dtype == QGEMM_F32;
   p.ep.act = a.act;
   p.ep.vec = aligned((uint64_t)a.out, 4 * os) && a.ldc % 4 == 0 &&
              (!a.residual || (aligned((uint64_t)a.residual, 4 * os) && a.ldr % 4 == 0));
@@ -1264,7 +1267,8 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
   const int avg = (a.M + groups - 1) / groups;
   p.seg_kb = SEG_KB;
   const bool seg = a.kind == KIND_BF16 && a.out_dtype == QGEMM_F32 && p.num_k_blocks > SEG_KB;
-  const int variant = a.kind == KIND_I8 ? 0 : seg ? 2 : 1;
+  const int f32 = a.out_dtype == QGEMM_F32;
+  const Kerns& kerns = a.kind == KIND_I8 ? kInt8[f32] : seg ? kBf16Seg : kBf16[f32];
   // ---- the streaming kernel's cut of the work ----
   const int cap = strm::TOK;
   int tok_max, box;
@@ -1362,7 +1366,7 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
     cfg.dynamicSmemBytes = (size_t)fixed + (size_t)p.stages * pair::STAGE_BYTES;
     cfg.gridDim = dim3(sms / 2 * 2);
     cfg.blockDim = dim3(pair::THREADS);
-    kern = kPair[variant][a.gated];
+    kern = kerns.pair[a.gated];
   } else {
     p.tok_max = tok_max;
     p.box = box;
@@ -1388,7 +1392,7 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
     const long long clusters = most < ds->clusters[pick] ? most : ds->clusters[pick];
     cfg.gridDim = dim3((unsigned)(clusters * p.csize));
     cfg.blockDim = dim3(strm::THREADS);
-    kern = kStream[variant][a.gated][p.csize > 1];
+    kern = kerns.stream[a.gated][p.csize > 1];
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = p.csize;
     attr[1].val.clusterDim.y = 1;

@@ -417,7 +417,11 @@ QGEMM_API qgemm_status qgemm_gemv_f32(qgemm_stream_t s, uint64_t A, uint64_t x, 
  *             layer then adds onto the stream in place)
  *   out       [M, ldc] of out_dtype (QGEMM_BF16 or QGEMM_F32); nothing past column N of a
  *             row is written
- * Everything is fp32 up to one rounding (RNE) to out_dtype.  bf16 sums run on the tensor
+ * Everything is fp32 up to one rounding (RNE) to out_dtype.  The activations are evaluated to
+ * a few units of 2^-24 of their result (SILU and GELU_TANH are 0 where exp passes e^87), but for
+ * SILU and GELU_TANH of bf16 outputs, whose exponentials are within (2 + 1.17 |v|) 2^-23 of
+ * themselves.
+ * bf16 sums run on the tensor
  * cores, whose fp32 additions truncate (about 1e-9 of the result a value of K, far below a
  * bf16 step); for fp32 outputs they are taken in pieces of 512 values that are added rounding
  * to nearest (about 5e-7, whatever K).  Deterministic: the same call

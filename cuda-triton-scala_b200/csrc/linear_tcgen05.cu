@@ -1160,18 +1160,19 @@ static constexpr Kerns kerns_of() {
 }
 static const Kerns kInt8[2] = {kerns_of<KIND_I8, false, false>(), kerns_of<KIND_I8, false, true>()};
 static const Kerns kBf16[2] = {kerns_of<KIND_BF16, false, false>(), kerns_of<KIND_BF16, false, true>()};
-static const Kerns kBf16Seg = kerns_of<KIND_BF16, true, true>();
-static const Kerns* const kAll[] = {&kInt8[0], &kInt8[1], &kBf16[0], &kBf16[1], &kBf16Seg};
+static const Kerns kBf16Seg[2] = {kerns_of<KIND_BF16, true, false>(), kerns_of<KIND_BF16, true, true>()};
+static const Kerns* const kAll[] = {&kInt8[0], &kInt8[1], &kBf16[0], &kBf16[1], &kBf16Seg[0], &kBf16Seg[1]};
 
 static_assert(pair::SEG_TOK <= 128 && 3 * strm::TOK <= 512, "TMEM columns of SEG");
 
 // The tensor cores add each MMA's products to the fp32 accumulator by truncation, so a sum
 // over K shrinks by about 9e-10 of itself a value of K (measured: 2.1e-6 at K = 2048, 1.2e-5 at
-// 11008).  bf16 outputs round 300 times coarser; fp32 outputs take the SEG kernels, which start
-// a new accumulator every SEG_KB k-blocks (512 values, 4.7e-7) and add the pieces rounding to
+// 11008).  A bf16 output's half step is 33 times that or more up to K = SEG_K; beyond, and for
+// fp32 outputs from the first, the SEG kernels run, which start a new accumulator every SEG_KB k-blocks (512 values, 4.7e-7) and add the pieces rounding to
 // nearest, into running sums in TMEM (in registers, the unrolled code ran from outside the
 // instruction cache: 170 us instead of 112 for 6001 x 1544 x 2048 over 64 experts).
 constexpr int SEG_KB = 8;
+constexpr int SEG_K = 65536;
 static_assert(SEG_KB % strm::STEP == 0, "a segment is whole stages");
 
 // Opts the kernels in to the whole shared memory once a device, and asks how many clusters of
@@ -1266,9 +1267,9 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
   const int groups = a.E < a.M ? a.E : a.M;
   const int avg = (a.M + groups - 1) / groups;
   p.seg_kb = SEG_KB;
-  const bool seg = a.kind == KIND_BF16 && a.out_dtype == QGEMM_F32 && p.num_k_blocks > SEG_KB;
   const int f32 = a.out_dtype == QGEMM_F32;
-  const Kerns& kerns = a.kind == KIND_I8 ? kInt8[f32] : seg ? kBf16Seg : kBf16[f32];
+  const bool seg = a.kind == KIND_BF16 && p.num_k_blocks > SEG_KB && (f32 || a.K > SEG_K);
+  const Kerns& kerns = a.kind == KIND_I8 ? kInt8[f32] : seg ? kBf16Seg[f32] : kBf16[f32];
   // ---- the streaming kernel's cut of the work ----
   const int cap = strm::TOK;
   int tok_max, box;

@@ -421,13 +421,15 @@ QGEMM_API qgemm_status qgemm_gemv_f32(qgemm_stream_t s, uint64_t A, uint64_t x, 
  * a few units of 2^-24 of their result (SILU and GELU_TANH are 0 where exp passes e^87), but for
  * SILU and GELU_TANH of bf16 outputs, whose exponentials are within (2 + 1.17 |v|) 2^-23 of
  * themselves.
- * bf16 sums run on the tensor
- * cores, whose fp32 additions truncate (about 1e-9 of the result a value of K, far below a
- * bf16 step); for fp32 outputs they are taken in pieces of 512 values that are added rounding
- * to nearest (about 5e-7, whatever K).  Deterministic: the same call
- * gives the same bits, whatever ran before.  Nothing is allocated and no scratch is used,
- * so calls on different streams, and captured graphs, are independent.  QGEMM_ALGO_AUTO
- * runs on the tensor cores when K is a multiple of 16 bytes and x, w and their rows are
+ * bf16 sums run on the tensor cores, whose fp32 additions truncate: a sum shrinks by about
+ * 9e-10 of itself a value of K, which for bf16 outputs is 1/33 of half a step at most up to
+ * K = 65536.  Beyond, and for fp32 outputs from K = 513 on, they are taken in pieces of 512
+ * values that are added rounding to nearest: 5e-7 of the result (measured up to K = 11008),
+ * at most (32 + K / 1024) 2^-23 of sum |x w|.  The CUDA cores add with k ascending, rounding to
+ * nearest (K 2^-24 of sum |x w| at most).
+ * Deterministic: the same call gives the same bits, whatever ran before.  Nothing is allocated
+ * and no scratch is used, so calls on different streams, and captured graphs, are independent.
+ * QGEMM_ALGO_AUTO runs on the tensor cores when K is a multiple of 16 bytes and x, w and their rows are
  * 16-byte aligned, else on CUDA cores (any K >= 0, any ldx; for odd shapes, not fast);
  * QGEMM_ALGO_TCGEN05 refuses what the tensor cores cannot take (QGEMM_ERR_UNSUPPORTED).
  * M == 0 or N == 0 does nothing.  int8: K <= 131071 (the int32 sums cannot overflow).

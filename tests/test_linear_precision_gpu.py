@@ -1,7 +1,8 @@
 """What an output keeps of its precision through each activation, far out on both sides.
 
-The bounds, relative to the exact value, with u = 2^-24 (the half step of fp32),
-expf within 2 ulp (4 u), erfcf within 4 ulp (8 u), 1 + e and the quotient within u each:
+The bounds are those of an evaluation by CUDA's functions, relative to the exact value, with
+u = 2^-24 (the half step of fp32), expf within 2 ulp (4 u), erfcf within 4 ulp (8 u), 1 + e and the
+quotient within u each:
   silu       v / (1 + exp(-v)): exp's error 4 u, the sum u, the quotient u: 6 u
   gelu       0.5 v erfc(x), x = -v / sqrt 2: the constant and the product err by u each, which
              erfc multiplies by |x erfc'(x) / erfc(x)| <= 2 x^2 + 1 = v^2 + 1 (x > 0; less than 1

@@ -22,7 +22,13 @@ struct qgemm_device_s {
   // (qgemm_debug_hold_split).
   unsigned long long wait_ns = 2000000000ull;
   int hold_split = 0;
-  std::mutex mu;
+  // Index-error words, one a stream handle (page-locked host memory that kernels write): the
+  // free ones wait in a ring, longest first, so that a word is not given out again while work
+  // of the handle that had it may still run.  Word 0 is shared by the handles past kIndexWords.
+  int* index_words = nullptr;
+  int* free_words = nullptr;
+  int free_first = 0, free_count = 0;
+  std::mutex mu;              // guards the ring
   bool open = false;
 };
 
@@ -36,6 +42,9 @@ struct qgemm_stream_s {
   // and grown (outside graph capture) when a call needs more.
   void* ws = nullptr;
   size_t ws_bytes = 0;
+  // Set by a kernel that met an expert offset or row index out of range (and skipped what it
+  // names); read and cleared by qgemm_stream_sync of this handle.
+  int* index_word = nullptr;
 };
 
 namespace qg {
@@ -60,10 +69,15 @@ enum : int {
   DEVERR_TIMEOUT_MMA = 2,
   DEVERR_TIMEOUT_EPILOGUE = 3,
   DEVERR_TIMEOUT_DRAIN = 4,
-  // An expert offset or row index read on the device lies outside its range; the kernel
-  // skipped what it names (reported as QGEMM_ERR_INVALID_ARG).
-  DEVERR_BAD_INDEX = 5,
 };
+constexpr int kIndexWords = 4096;
+
+#ifdef __CUDACC__
+// Notes an index out of range in a stream handle's index_word.
+__device__ __forceinline__ void note_bad_index(int* word) {
+  *static_cast<volatile int*>(word) = 1;
+}
+#endif
 
 // ---- the tcgen05 GEMM (w8a8_tcgen05.cu) ----
 // MMA kinds of the tcgen05 GEMM kernels.

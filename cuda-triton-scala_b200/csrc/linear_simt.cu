@@ -34,7 +34,7 @@ template <> struct Elem<KIND_BF16> {
 };
 
 template <int KIND, bool GATED>
-__global__ void __launch_bounds__(256) linear_simt_kernel(const LinArgs a, Epi ep, int* err) {
+__global__ void __launch_bounds__(256) linear_simt_kernel(const LinArgs a, Epi ep, int* bad) {
   using El = Elem<KIND>;
   using Acc = typename El::Acc;
   const auto* x = static_cast<const typename El::T*>(a.x);
@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(256) linear_simt_kernel(const LinArgs a, Epi e
       for (int e = 0; e < a.E; ++e) {
         const int o0 = a.offsets[e], o1 = a.offsets[e + 1];
         if (o0 < 0 || o1 < o0 || o1 > a.M) {
-          if (err) atomicCAS(err, 0, DEVERR_BAD_INDEX);
+          note_bad_index(bad);
           continue;
         }
         const int tiles = (o1 - o0 + TM - 1) / TM;
@@ -127,13 +127,13 @@ qgemm_status launch_linear_simt(qgemm_stream_s* s, const LinArgs& a) {
   if (row_tiles > 65535)
     return fail(QGEMM_ERR_UNSUPPORTED, "M %d is too large for the CUDA-core path", a.M);
   const dim3 grid((a.N + TN - 1) / TN, (unsigned)row_tiles);
-  int* err = s->dev->d_err;
+  int* bad = s->index_word;
   if (a.kind == KIND_I8) {
-    if (a.gated) linear_simt_kernel<KIND_I8, true><<<grid, 256, 0, s->stream>>>(a, ep, err);
-    else linear_simt_kernel<KIND_I8, false><<<grid, 256, 0, s->stream>>>(a, ep, err);
+    if (a.gated) linear_simt_kernel<KIND_I8, true><<<grid, 256, 0, s->stream>>>(a, ep, bad);
+    else linear_simt_kernel<KIND_I8, false><<<grid, 256, 0, s->stream>>>(a, ep, bad);
   } else {
-    if (a.gated) linear_simt_kernel<KIND_BF16, true><<<grid, 256, 0, s->stream>>>(a, ep, err);
-    else linear_simt_kernel<KIND_BF16, false><<<grid, 256, 0, s->stream>>>(a, ep, err);
+    if (a.gated) linear_simt_kernel<KIND_BF16, true><<<grid, 256, 0, s->stream>>>(a, ep, bad);
+    else linear_simt_kernel<KIND_BF16, false><<<grid, 256, 0, s->stream>>>(a, ep, bad);
   }
   return cuda_fail(cudaGetLastError(), "linear_simt launch");
 }

@@ -68,7 +68,8 @@ struct Params {
   int csize;        // CTAs of a cluster (stream kernel)
   int box;          // token rows of a TMA box (stream kernel)
   int tmem_cols;    // TMEM columns (stream kernel)
-  int* err;
+  int* err;         // a wait ran out
+  int* bad;         // an offset out of range
   unsigned long long wait_ns;
 };
 
@@ -101,7 +102,7 @@ __device__ __forceinline__ void fill_table(const Params& p, const Table& tb) {
   for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
     int o0 = p.offsets[e], o1 = p.offsets[e + 1];
     if (o0 < 0 || o1 < o0 || o1 > p.M) {
-      if (p.err && blockIdx.x == 0) atomicCAS(p.err, 0, DEVERR_BAD_INDEX);
+      if (blockIdx.x == 0) note_bad_index(p.bad);
       o0 = o1 = 0;
     }
     tb.row0[e] = o0;
@@ -1260,6 +1261,7 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
   p.E = a.E; p.M = a.M;
   p.num_k_blocks = (int)(((long long)a.K * es + BK - 1) / BK);
   p.err = s->dev->d_err;
+  p.bad = s->index_word;
   p.wait_ns = s->dev->wait_ns;
   p.rows = WROWS;
   const int table = ((3 * a.E + 1) * 4 + 15) / 16 * 16;

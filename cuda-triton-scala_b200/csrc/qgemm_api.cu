@@ -162,9 +162,25 @@ qgemm_status qgemm_device_open(int ordinal, qgemm_device_t* out) {
   e = cudaMalloc(&d->d_err, 256);
   if (e == cudaSuccess) e = cudaMemset(d->d_err, 0, 256);
   if (e != cudaSuccess) {
+    if (d->d_err) cudaFree(d->d_err);
     delete d;
     return cuda_fail(e, "device error word");
   }
+  void* words = nullptr;
+  e = cudaHostAlloc(&words, kIndexWords * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
+  d->free_words = new (std::nothrow) int[kIndexWords];
+  if (e != cudaSuccess || !d->free_words) {
+    if (e == cudaSuccess) cudaFreeHost(words);
+    cudaFree(d->d_err);
+    delete[] d->free_words;
+    delete d;
+    return e != cudaSuccess ? cuda_fail(e, "index-error words")
+                            : fail(QGEMM_ERR_OOM, "host allocation failed");
+  }
+  d->index_words = static_cast<int*>(words);
+  memset(words, 0, kIndexWords * sizeof(int));
+  for (int i = 1; i < kIndexWords; ++i) d->free_words[i - 1] = i;
+  d->free_count = kIndexWords - 1;
   d->open = true;
   *out = d;
   return QGEMM_OK;
@@ -174,6 +190,8 @@ qgemm_status qgemm_device_close(qgemm_device_t d) {
   if (!d || !d->open) return fail(QGEMM_ERR_BAD_HANDLE, "null or closed device");
   cudaSetDevice(d->ordinal);
   cudaFree(d->d_err);
+  cudaFreeHost(d->index_words);
+  delete[] d->free_words;
   d->open = false;
   delete d;
   return QGEMM_OK;
@@ -214,6 +232,27 @@ qgemm_status qgemm_debug_hold_split(qgemm_device_t d, int enable) {
 
 // ---- streams ----
 
+// Gives a handle its index-error word, clean; and back.
+static void take_index_word(qgemm_stream_s* s) {
+  qgemm_device_s* d = s->dev;
+  std::lock_guard<std::mutex> lock(d->mu);
+  int i = 0;
+  if (d->free_count > 0) {
+    i = d->free_words[d->free_first];
+    d->free_first = (d->free_first + 1) % kIndexWords;
+    --d->free_count;
+    static_cast<volatile int*>(d->index_words)[i] = 0;
+  }
+  s->index_word = d->index_words + i;
+}
+
+static void return_index_word(qgemm_stream_s* s) {
+  qgemm_device_s* d = s->dev;
+  std::lock_guard<std::mutex> lock(d->mu);
+  const int i = (int)(s->index_word - d->index_words);
+  if (i > 0) d->free_words[(d->free_first + d->free_count++) % kIndexWords] = i;
+}
+
 qgemm_status qgemm_stream_create(qgemm_device_t d, qgemm_stream_t* out) {
   if (!out) return fail(QGEMM_ERR_INVALID_ARG, "out is null");
   if (!d || !d->open) return fail(QGEMM_ERR_BAD_HANDLE, "null or closed device");
@@ -230,6 +269,7 @@ qgemm_status qgemm_stream_create(qgemm_device_t d, qgemm_stream_t* out) {
   s->dev = d;
   s->stream = st;
   s->owned = true;
+  take_index_word(s);
   *out = s;
   return QGEMM_OK;
 }
@@ -242,6 +282,7 @@ qgemm_status qgemm_stream_wrap(qgemm_device_t d, void* cuda_stream, qgemm_stream
   s->dev = d;
   s->stream = static_cast<cudaStream_t>(cuda_stream);
   s->owned = false;
+  take_index_word(s);
   *out = s;
   return QGEMM_OK;
 }
@@ -256,6 +297,7 @@ qgemm_status qgemm_stream_destroy(qgemm_stream_t s) {
       cudaFree(s->ws);
     }
     if (s->owned) cudaStreamDestroy(s->stream);
+    return_index_word(s);
   }
   delete s;
   return QGEMM_OK;
@@ -276,10 +318,13 @@ qgemm_status qgemm_stream_sync(qgemm_stream_t s) {
     // a kernel that gave up may have left split-tile counters raised
     if (s->ws) cudaMemsetAsync(s->ws, 0, s->ws_bytes, s->stream);
     cudaStreamSynchronize(s->stream);
-    if (err == DEVERR_BAD_INDEX)
-      return fail(QGEMM_ERR_INVALID_ARG,
-                  "an expert offset or row index read on the device was out of range");
     return fail(QGEMM_ERR_TIMEOUT, "a device-side wait ran out (code %d)", err);
+  }
+  volatile int* const bad = s->index_word;
+  if (*bad) {
+    *bad = 0;
+    return fail(QGEMM_ERR_INVALID_ARG,
+                "an expert offset or row index read on the device was out of range");
   }
   return QGEMM_OK;
 }

@@ -277,7 +277,7 @@ template <typename V>
 __global__ void __launch_bounds__(256) dispatch_copy_kernel(const V* __restrict__ x,
                                                             const int* __restrict__ rows,
                                                             V* __restrict__ out, int T, int k,
-                                                            int pieces, int R, int* err) {
+                                                            int pieces, int R, int* bad) {
   ptx::grid_launch_dependents();
   ptx::grid_dependency_wait();
   const int c = blockIdx.x * 256 + threadIdx.x;
@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(256) dispatch_copy_kernel(const V* __restrict_
     for (int j = 0; j < k; ++j) {
       const int r = __ldg(rows + (size_t)t * k + j);
       if (r >= R) {
-        if (c == 0) atomicCAS(err, 0, DEVERR_BAD_INDEX);
+        if (c == 0) note_bad_index(bad);
       } else if (r >= 0) {
         out[(size_t)r * pieces + c] = v;
       }
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(256) dispatch_quant_kernel(const T* __restrict
                                                              const int* __restrict__ rows,
                                                              int8_t* __restrict__ q,
                                                              float* __restrict__ sA, int k, int K,
-                                                             int R, int* err) {
+                                                             int R, int* bad) {
   ptx::grid_launch_dependents();
   ptx::grid_dependency_wait();
   const int t = blockIdx.x;
@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(256) dispatch_quant_kernel(const T* __restrict
     const int r = __ldg(rows + (size_t)t * k + j);
     if (r < 0) continue;
     if (r >= R) {
-      if (tid == 0) atomicCAS(err, 0, DEVERR_BAD_INDEX);
+      if (tid == 0) note_bad_index(bad);
       continue;
     }
     if (tid == 0) sA[r] = scale;
@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const TI* __restrict__ y,
                                                       const int* __restrict__ rows,
                                                       const float* __restrict__ weights,
                                                       const TO* residual, TO* out, int T, int k,
-                                                      int N, int R, int* err) {
+                                                      int N, int R, int* bad) {
   constexpr int RAW = VEC ? (int)sizeof(TI) / 2 : 1;  // 16-byte words of 8 elements
   ptx::grid_launch_dependents();
   ptx::grid_dependency_wait();
@@ -463,7 +463,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const TI* __restrict__ y,
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (row[u] >= R) {
-          if (c == 0) atomicCAS(err, 0, DEVERR_BAD_INDEX);
+          if (c == 0) note_bad_index(bad);
           row[u] = -1;
         }
         if constexpr (VEC) {
@@ -598,15 +598,15 @@ cudaError_t quant_t(qgemm_stream_s* s, const T* x, const int* rows, int8_t* q, f
                     int k, int K, int R) {
   const bool vec = K % 4 == 0 && aligned((uint64_t)x, 4 * sizeof(T)) && aligned((uint64_t)q, 4);
   const int nv = vec ? (K / 4 + 255) / 256 : 0;
-  int* err = s->dev->d_err;
+  int* bad = s->index_word;
   const dim3 g(n);
-  if (nv == 1) return launch(dispatch_quant_kernel<T, 1>, g, 256, 0, s->stream, 1, x, rows, q, sA, k, K, R, err);
-  if (nv == 2) return launch(dispatch_quant_kernel<T, 2>, g, 256, 0, s->stream, 1, x, rows, q, sA, k, K, R, err);
+  if (nv == 1) return launch(dispatch_quant_kernel<T, 1>, g, 256, 0, s->stream, 1, x, rows, q, sA, k, K, R, bad);
+  if (nv == 2) return launch(dispatch_quant_kernel<T, 2>, g, 256, 0, s->stream, 1, x, rows, q, sA, k, K, R, bad);
   if (nv == 3 || nv == 4)
-    return launch(dispatch_quant_kernel<T, 4>, g, 256, 0, s->stream, 1, x, rows, q, sA, k, K, R, err);
+    return launch(dispatch_quant_kernel<T, 4>, g, 256, 0, s->stream, 1, x, rows, q, sA, k, K, R, bad);
   if (nv > 4 && nv <= 8)
-    return launch(dispatch_quant_kernel<T, 8>, g, 256, 0, s->stream, 1, x, rows, q, sA, k, K, R, err);
-  return launch(dispatch_quant_kernel<T, 0>, g, 256, 0, s->stream, 1, x, rows, q, sA, k, K, R, err);
+    return launch(dispatch_quant_kernel<T, 8>, g, 256, 0, s->stream, 1, x, rows, q, sA, k, K, R, bad);
+  return launch(dispatch_quant_kernel<T, 0>, g, 256, 0, s->stream, 1, x, rows, q, sA, k, K, R, bad);
 }
 
 template <typename V>
@@ -614,7 +614,7 @@ cudaError_t copy_t(qgemm_stream_s* s, const void* x, const int* rows, void* out,
                    int pieces, int R) {
   const dim3 g((pieces + 255) / 256, n < 65535 ? n : 65535);
   return launch(dispatch_copy_kernel<V>, g, 256, 0, s->stream, 1, static_cast<const V*>(x), rows,
-                static_cast<V*>(out), n, k, pieces, R, s->dev->d_err);
+                static_cast<V*>(out), n, k, pieces, R, s->index_word);
 }
 
 template <typename TI, typename TO>
@@ -626,9 +626,9 @@ cudaError_t combine_t(qgemm_stream_s* s, const void* y, const int* rows, const f
   const TI* yi = static_cast<const TI*>(y);
   const TO* ri = static_cast<const TO*>(residual);
   TO* o = static_cast<TO*>(out);
-  int* err = s->dev->d_err;
+  int* bad = s->index_word;
   auto go = [&](auto kern) {
-    return launch(kern, g, 128, 0, s->stream, 1, yi, rows, weights, ri, o, n, k, N, R, err);
+    return launch(kern, g, 128, 0, s->stream, 1, yi, rows, weights, ri, o, n, k, N, R, bad);
   };
   if (!vec) return go(combine_kernel<TI, TO, false, 2>);
   if (k <= 2) return go(combine_kernel<TI, TO, true, 2>);

@@ -129,7 +129,12 @@ QGEMM_API qgemm_status qgemm_stream_create(qgemm_device_t dev, qgemm_stream_t* o
 /* Adopt a caller-owned cudaStream_t (not destroyed by qgemm_stream_destroy). */
 QGEMM_API qgemm_status qgemm_stream_wrap(qgemm_device_t dev, void* cuda_stream, qgemm_stream_t* out);
 QGEMM_API qgemm_status qgemm_stream_destroy(qgemm_stream_t s);
-/* Synchronise, then report (and clear) a device-side timeout on this device. */
+/* Synchronise, then report (and clear) a device-side timeout on this device (QGEMM_ERR_TIMEOUT),
+ * else an offset or row index out of range that a call on this handle read on the device
+ * (QGEMM_ERR_INVALID_ARG): that one goes to the handle that made the call, and where both
+ * happened it is left for the next sync.  Replays of a captured graph report to the handle
+ * that captured it, which has to live as long (more than 4095 handles open at a time on a
+ * device share the last word). */
 QGEMM_API qgemm_status qgemm_stream_sync(qgemm_stream_t s);
 
 /* ---- buffers ---------------------------------------------------------------
@@ -451,7 +456,7 @@ QGEMM_API qgemm_status qgemm_w8a8_linear(qgemm_stream_t s, uint64_t A, int lda, 
  *             qgemm_route_topk; read by the kernel, so the host need not know the counts
  * M is the number of rows that x and out have; rows outside every expert (past offsets[E])
  * are not written.  An expert may have no rows.  Offsets that break the rule above name no
- * rows (that expert is skipped) and the next qgemm_stream_sync reports
+ * rows (that expert is skipped) and the next qgemm_stream_sync of this handle reports
  * QGEMM_ERR_INVALID_ARG. */
 QGEMM_API qgemm_status qgemm_expert_linear_bf16_nk(qgemm_stream_t s, uint64_t x, int ldx,
                                                    uint64_t w, uint64_t bias, uint64_t offsets,
@@ -489,7 +494,7 @@ QGEMM_API qgemm_status qgemm_w8a8_expert_linear(qgemm_stream_t s, uint64_t A, in
  * all one; residual 0: none (it may be `out` itself).
  *
  * rows[t,j] < 0 names no row (nothing is written, nothing added); a row >= R is skipped and
- * the next qgemm_stream_sync reports QGEMM_ERR_INVALID_ARG.  Two pairs that name one row
+ * the next qgemm_stream_sync of this handle reports QGEMM_ERR_INVALID_ARG.  Two pairs that name one row
  * leave either's values there.  Outputs may not overlap inputs, but for the residual. */
 QGEMM_API qgemm_status qgemm_route_topk(qgemm_stream_t s, uint64_t logits, int in_dtype,
                                         uint64_t weights, uint64_t experts, uint64_t offsets,

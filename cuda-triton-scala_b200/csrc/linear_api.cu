@@ -39,12 +39,18 @@ qgemm_status dtype_ok(int t, const char* name) {
   return QGEMM_OK;
 }
 
+// Rows, features and values a row at most: loops and tile counts of the kernels step past the end
+// by up to a block's width in 32 bits.
+constexpr int kMostSize = 1 << 30;
+
 qgemm_status linear_entry(qgemm_stream_t s, int kind, uint64_t x, int ldx, uint64_t w,
                           uint64_t sx, uint64_t sw, uint64_t bias, uint64_t residual, int ldr,
                           uint64_t offsets, bool experts, uint64_t out, int out_dtype, int ldc,
                           int E, int M, int N, int K, int act, int gated, int algo) {
   if (M < 0 || N < 0 || K < 0)
     return fail(QGEMM_ERR_INVALID_ARG, "negative size M=%d N=%d K=%d", M, N, K);
+  if (M > kMostSize || N > kMostSize || K > kMostSize)
+    return fail(QGEMM_ERR_UNSUPPORTED, "size past 2^30: M=%d N=%d K=%d", M, N, K);
   if (E < 1 || E > kMaxExperts)
     return fail(QGEMM_ERR_INVALID_ARG, "E %d outside [1, %d]", E, kMaxExperts);
   QG_TRY(dtype_ok(out_dtype, "out_dtype"));
@@ -115,6 +121,8 @@ qgemm_status rows_entry(qgemm_stream_t s, int in_dtype, int T, int k, int W, int
   if (k < 1 || k > 64) return fail(QGEMM_ERR_INVALID_ARG, "k %d outside [1, 64]", k);
   if ((long long)T * k > 0x7fffffffll)
     return fail(QGEMM_ERR_UNSUPPORTED, "T * k exceeds 2^31 - 1");
+  if (T > kMostSize || W > kMostSize)
+    return fail(QGEMM_ERR_UNSUPPORTED, "size past 2^30: T=%d %s=%d", T, width, W);
   return dtype_ok(in_dtype, "in_dtype");
 }
 
@@ -166,6 +174,7 @@ qgemm_status qgemm_route_topk(qgemm_stream_t s, uint64_t logits, int in_dtype, u
     return fail(QGEMM_ERR_INVALID_ARG, "renormalize %d is not 0 or 1", renormalize);
   if ((long long)T * k > 0x7fffffffll)
     return fail(QGEMM_ERR_UNSUPPORTED, "T * k exceeds 2^31 - 1");
+  if (T > kMostSize) return fail(QGEMM_ERR_UNSUPPORTED, "size past 2^30: T=%d", T);
   QG_TRY(dtype_ok(in_dtype, "in_dtype"));
   QG_TRY(need(offsets, 4, "offsets"));
   if (T > 0) {

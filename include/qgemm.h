@@ -437,7 +437,7 @@ QGEMM_API qgemm_status qgemm_gemv_f32(qgemm_stream_t s, uint64_t A, uint64_t x, 
  * QGEMM_ALGO_AUTO runs on the tensor cores when K is a multiple of 16 bytes and x, w and their rows are
  * 16-byte aligned, else on CUDA cores (any K >= 0, any ldx; for odd shapes, not fast);
  * QGEMM_ALGO_TCGEN05 refuses what the tensor cores cannot take (QGEMM_ERR_UNSUPPORTED).
- * M == 0 or N == 0 does nothing.  int8: K <= 131071 (the int32 sums cannot overflow).
+ * M == 0 or N == 0 does nothing.  M, N, K <= 2^30.  int8: K <= 131071 (the int32 sums cannot overflow).
  * `out` may not overlap x, w, or (unless it is the same buffer) the residual. */
 QGEMM_API qgemm_status qgemm_linear_bf16_nk(qgemm_stream_t s, uint64_t x, int ldx, uint64_t w,
                                             uint64_t bias, uint64_t residual, int ldr,
@@ -470,7 +470,8 @@ QGEMM_API qgemm_status qgemm_w8a8_expert_linear(qgemm_stream_t s, uint64_t A, in
                                                 int gated, int algo);
 
 /* ---- tokens to experts and back --------------------------------------------
- * The steps around the expert layers.  T tokens, k experts each; R = T * k rows.
+ * The steps around the expert layers.  T tokens, k experts each; R = T * k rows.  T and the
+ * values of a row <= 2^30, T * k < 2^31.
  *
  * qgemm_route_topk: for each token the k experts with the largest logits (a tie goes to
  * the lower index), in descending order, and their softmax weights: over all E logits, or

@@ -38,6 +38,7 @@
 #include <mutex>
 
 #include "linear_epilogue.cuh"
+#include "linear_tiles.cuh"
 #include "ptx.cuh"
 
 namespace qg {
@@ -52,15 +53,10 @@ constexpr int SMEM_MAX = 232448;             // 227 KB
 constexpr int BAR_BYTES = 640;
 constexpr int MAX_STAGES = 32;
 
-struct Params {
+struct Params : Schedule {
   Epi ep;
   const int* offsets;
-  int E, M;
   int num_k_blocks;
-  int tok_max;      // tokens of a tile at most
-  int tok_round;    // tokens of a tile are a multiple of this (MMA N)
-  int num_w_blocks; // weight blocks of an expert
-  int band;         // token blocks of a band of the schedule
   int rows;         // weight rows of a CTA's tile: 128, in the stream kernel a multiple of 16
   int feats;        // features of them: rows, gated rows / 2
   int stages;
@@ -73,22 +69,6 @@ struct Params {
   unsigned long long wait_ns;
 };
 
-// The experts' rows and tiles, in shared memory.
-struct Table {
-  int* row0;  // [E] first row
-  int* cnt;   // [E] rows (0 where the offsets are not usable)
-  int* pref;  // [E + 1] tiles before the expert
-};
-
-struct Tile {
-  int e, wb;   // expert, weight block
-  int t0, n;   // first row of x / out, rows
-};
-
-__device__ __forceinline__ int blocks_of(const Params& p, int cnt) {
-  return (cnt + p.tok_max - 1) / p.tok_max;
-}
-
 // One thread: the table of a dense layer, one group of M rows.
 __device__ __forceinline__ void dense_table(const Params& p, const Table& tb) {
   tb.row0[0] = 0;
@@ -97,14 +77,11 @@ __device__ __forceinline__ void dense_table(const Params& p, const Table& tb) {
   tb.pref[1] = blocks_of(p, p.M) * p.num_w_blocks;
 }
 
-// All threads: fills the experts' table.  Offsets that are not 0 <= o[e] <= o[e+1] <= M name no rows.
+// All threads: fills the experts' table.  No rows where expert_rows or kMostTiles says so.
 __device__ __forceinline__ void fill_table(const Params& p, const Table& tb) {
   for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
-    int o0 = p.offsets[e], o1 = p.offsets[e + 1];
-    if (o0 < 0 || o1 < o0 || o1 > p.M) {
-      if (blockIdx.x == 0) note_bad_index(p.bad);
-      o0 = o1 = 0;
-    }
+    int o0, o1;
+    if (!expert_rows(p, p.offsets, e, o0, o1) && blockIdx.x == 0) note_bad_index(p.bad);
     tb.row0[e] = o0;
     tb.cnt[e] = o1 - o0;
     tb.pref[e] = blocks_of(p, o1 - o0) * p.num_w_blocks;
@@ -113,52 +90,25 @@ __device__ __forceinline__ void fill_table(const Params& p, const Table& tb) {
   if (threadIdx.x < 32) {  // exclusive scan, a run of experts a lane
     const int lane = threadIdx.x;
     const int chunk = (p.E + 31) / 32, e0 = min(p.E, lane * chunk), e1 = min(p.E, e0 + chunk);
-    int sum = 0;
+    long long sum = 0;
     for (int e = e0; e < e1; ++e) sum += tb.pref[e];
-    int run = sum;
+    long long run = sum;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-      const int o = __shfl_up_sync(0xffffffffu, run, off);
+      const long long o = __shfl_up_sync(0xffffffffu, run, off);
       if (lane >= off) run += o;
     }
-    if (lane == 31) tb.pref[p.E] = run;
+    const long long all = __shfl_sync(0xffffffffu, run, 31);
+    if (all > kMostTiles && lane == 0 && blockIdx.x == 0) note_bad_index(p.bad);
+    if (lane == 31) tb.pref[p.E] = tiles_before(all, all);
     run -= sum;
     for (int e = e0; e < e1; ++e) {
       const int c = tb.pref[e];
-      tb.pref[e] = run;
+      tb.pref[e] = tiles_before(run, all);
       run += c;
     }
   }
   __syncthreads();
-}
-
-// Tile `t` of the schedule.  An expert's rows are cut into blocks of equal size (rounded up
-// to tok_round).  Order inside an expert: bands of `band` token blocks; in a band the token
-// block runs fastest, so CTAs that work at the same time share weights and tokens in L2.
-__device__ __forceinline__ Tile tile_of(const Params& p, const Table& tb, int t, int band) {
-  int e = 0;
-  if (p.E > 1) {  // the last expert whose first tile is <= t (experts without rows have none)
-    int lo = 0, hi = p.E;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (tb.pref[mid] <= t) lo = mid; else hi = mid;
-    }
-    e = lo;
-  }
-  const int idx = t - tb.pref[e], cnt = tb.cnt[e];
-  const int nblk = blocks_of(p, cnt);
-  const int blk = (((cnt + nblk - 1) / nblk) + p.tok_round - 1) / p.tok_round * p.tok_round;
-  band = min(band, nblk);
-  const int per_band = band * p.num_w_blocks;
-  const int b = idx / per_band, in = idx - b * per_band;
-  const int rows = min(nblk - b * band, band);
-  Tile r;
-  r.e = e;
-  r.wb = in / rows;
-  const int first = (b * band + in % rows) * blk;
-  r.t0 = tb.row0[e] + first;
-  r.n = max(0, min(blk, cnt - first));
-  return r;
 }
 
 __device__ __forceinline__ void report(int* err, int code, volatile int* abort_flag) {
@@ -454,30 +404,6 @@ constexpr int EPI_WARPS = 8;              // two groups of four (one warp a TMEM
 constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr int SEG_TOK = 128;              // tokens of a tile at most with SEG
 }  // namespace pair
-
-// Item i of pair `pid`: a whole tile in the full rounds; in the last round the `rest` tiles
-// that are left are cut along their tokens into up to four parts, one a pair, so that the
-// round takes a part's time.  Returns false when there is none; an item may have no tokens.
-__device__ __forceinline__ bool pair_item(const Params& p, const Table& tb, int pid, int npairs,
-                                          int i, Tile& r) {
-  const int T = tb.pref[p.E];
-  const int rounds = T / npairs, rest = T - rounds * npairs;
-  if (i < rounds) {
-    r = tile_of(p, tb, pid + i * npairs, p.band);
-    return true;
-  }
-  if (i > rounds || rest == 0) return false;
-  const int parts = min(4, npairs / rest);
-  if (pid >= rest * parts) return false;
-  r = tile_of(p, tb, rounds * npairs + pid / parts, p.band);
-  if (parts > 1) {
-    const int w = ((r.n + parts - 1) / parts + p.tok_round - 1) / p.tok_round * p.tok_round;
-    const int first = (pid % parts) * w;
-    r.n = max(0, min(w, r.n - first));
-    r.t0 += first;
-  }
-  return true;
-}
 
 // F32: the output's type (and the residual's), and with it the form of the activation.
 template <int KIND, bool GATED, bool SEG, bool F32>

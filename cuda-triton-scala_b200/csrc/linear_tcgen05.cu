@@ -28,8 +28,11 @@
 // shared memory (prefix sums) and walks the same persistent schedule, so the host never
 // waits for the counts.
 //
-// Every barrier wait is bounded; one that runs out records a code in the device error word
-// and the CTA drains its copies and MMAs, frees TMEM and returns.
+// Every barrier wait is bounded; one that runs out records a code in the device error word, and
+// the abort flags that it raises make every other wait of the cluster give up.  Then, once all
+// warps have stopped issuing, the CTA waits for its copies and MMAs (and, where K is cut, for the
+// exchange's copies) whoever gave up, frees TMEM and returns.  Those waits have a limit of their
+// own: the device's may be too short for a copy to land.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -64,6 +67,7 @@ struct Params : Schedule {
   int csize;        // CTAs of a cluster (stream kernel)
   int box;          // token rows of a TMA box (stream kernel)
   int tmem_cols;    // TMEM columns (stream kernel)
+  int hold;         // the epilogue waits for what never comes (qgemm_debug_hold_split)
   int* err;         // a wait ran out
   int* bad;         // an offset out of range
   unsigned long long wait_ns;
@@ -110,6 +114,9 @@ __device__ __forceinline__ void fill_table(const Params& p, const Table& tb) {
   }
   __syncthreads();
 }
+
+// Limit of the waits for this CTA's own copies and MMAs after it has given up.
+constexpr unsigned long long DRAIN_NS = ptx::kWaitLimitNs;
 
 __device__ __forceinline__ void report(int* err, int code, volatile int* abort_flag) {
   *abort_flag = 1;
@@ -405,6 +412,50 @@ constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr int SEG_TOK = 128;              // tokens of a tile at most with SEG
 }  // namespace pair
 
+// What a pair that gave up has under way, once neither CTA issues any more and both see their
+// abort flag; all threads of both.  (Out of line, as the stream kernel's: inline it lay between
+// the hot code and the exit, and cost small calls 0.3 us of instruction fetch.)
+namespace pair {
+__device__ __noinline__ void drain(const Params& p, uint32_t base, const uint8_t* gbar, int count_at,
+                                   int boxes_at, uint32_t drain_bar, volatile int* abort_flag) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, S = p.stages;
+  const uint32_t rank = ptx::cluster_ctarank();
+  auto full_bar = [&](int s) { return base + S * STAGE_BYTES + 8u * s; };
+  if (warp == 0 && rank == 0 && lane == 0) {
+    // The even CTA's full barriers count both CTAs' copies.  Where one producer got further than
+    // the other, the missing half of a stage is taken off its count (the even CTA armed it for
+    // both), or the half that is on its way armed alone.
+    const uint32_t there = ptx::map_to_rank(base + S * STAGE_BYTES, 1);
+    const long long mine = *reinterpret_cast<const volatile long long*>(gbar + count_at);
+    const long long theirs = ptx::ld_cluster_s64(there + count_at);
+    const long long first = min(mine, theirs), end = max(mine, theirs);
+    for (long long f = first; f < end; ++f) {
+      const int at = (int)(f % S);
+      const uint32_t boxes = mine > theirs ? (uint32_t)gbar[boxes_at + at]
+                                           : ptx::ld_cluster_u8(there + boxes_at + at);
+      const uint32_t half = W_BYTES + boxes * BOX * BK;
+      if (mine > theirs) ptx::mbar_complete_tx(full_bar(at), half);
+      else ptx::mbar_arrive_expect_tx(full_bar(at), half);
+    }
+    for (long long f = max(0ll, end - S); f < end; ++f)
+      if (!ptx::mbar_wait(full_bar((int)(f % S)), (uint32_t)((f / S) & 1), nullptr, DRAIN_NS)) {
+        report(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag);
+        break;
+      }
+  }
+  __syncwarp();
+  if (warp == 1) {  // everything that the even CTA's issuer has committed, in both CTAs
+    if (rank == 0 && ptx::elect_one()) ptx::umma_commit_pair(drain_bar, 0x3);
+    __syncwarp();
+    if (lane == 0 && !ptx::mbar_wait(drain_bar, 0, nullptr, DRAIN_NS))
+      report(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag);
+    __syncwarp();
+  }
+  __syncthreads();
+  ptx::cluster_sync_all();  // neither CTA leaves before the other's copies and MMAs have ended
+}
+}  // namespace pair
+
 // F32: the output's type (and the residual's), and with it the form of the activation.
 template <int KIND, bool GATED, bool SEG, bool F32>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
@@ -426,6 +477,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
   const uint32_t drain_bar = bar_base + 8u * (2 * MAX_STAGES + 4);
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gbar + 8 * (2 * MAX_STAGES + 5));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gbar + 8 * (2 * MAX_STAGES + 5) + 4);
+  // stages this CTA's producer filled, and the token boxes of the last one in each place: what
+  // the drain needs of both CTAs
+  constexpr int COUNT_AT = 8 * (2 * MAX_STAGES + 6), BOXES_AT = COUNT_AT + 8;
+  static_assert(BOXES_AT + MAX_STAGES <= BAR_BYTES, "barriers and counts");
   Table tb;
   tb.row0 = reinterpret_cast<int*>(gbar + BAR_BYTES);
   tb.cnt = tb.row0 + p.E;
@@ -486,6 +541,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
           break;
         }
         if (ptx::elect_one()) {
+          gbar[BOXES_AT + stage] = (uint8_t)boxes;
           const uint32_t sw = base + stage * pair::STAGE_BYTES, sx = sw + W_BYTES;
           const uint32_t fb = ptx::map_to_rank(full_bar(stage), 0);
           if (rank == 0) ptx::mbar_arrive_expect_tx(full_bar(stage), tx);
@@ -517,23 +573,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
         if (++stage == S) { stage = 0; phase ^= 1u; }
       }
     }
-    // Drain: the even CTA's full barriers count both CTAs' copies.
-    if (rank == 0 && lane == 0) {
-      for (long long f = (issued > S ? issued - S : 0); f < issued; ++f) {
-        if (!ptx::mbar_wait(full_bar((int)(f % S)), (uint32_t)((f / S) & 1), nullptr, p.wait_ns)) {
-          report_cluster(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag, 2);
-          break;
-        }
-      }
-    }
-    __syncwarp();
+    if (lane == 0) *reinterpret_cast<volatile long long*>(gbar + COUNT_AT) = issued;
   } else if (warp == 1) {
     // ---------------- MMA issuer (even CTA) ----------------
     if (rank == 0) {
       int stage = 0;
       uint32_t phase = 0;
       int it = 0;
-      bool ok = true, issued_any = false;
+      bool ok = true;
       for (int item = 0; ok && pair_item(p, tb, pid, npairs, item, it_); ++item) {
         if (it_.n == 0) continue;
         const int ncol = (it_.n + p.tok_round - 1) / p.tok_round * p.tok_round;
@@ -573,17 +620,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
               if (kb + 1 == kb1) ptx::umma_commit_pair(tfull_bar(a), 0x3);
             }
             __syncwarp();
-            issued_any = true;
             if (++stage == S) { stage = 0; phase ^= 1u; }
           }
         }
-      }
-      if (!ok && issued_any) {
-        if (ptx::elect_one()) ptx::umma_commit_pair(drain_bar, 0x1);
-        __syncwarp();
-        if (lane == 0 && !ptx::mbar_wait(drain_bar, 0, nullptr, p.wait_ns))
-          report_cluster(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag, 2);
-        __syncwarp();
       }
     }
   } else {
@@ -610,7 +649,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
       }
       // Waits for accumulator it & 1; a warp whose wait ran out stores nothing.
       auto acc_ready = [&]() {
-        bool ok = ptx::mbar_wait(tfull_bar(it & 1), (uint32_t)((it >> 1) & 1), abort_flag, p.wait_ns);
+        bool ok = ptx::mbar_wait(p.hold ? drain_bar : tfull_bar(it & 1),
+                                 p.hold ? 0u : (uint32_t)((it >> 1) & 1), abort_flag, p.wait_ns);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok && lane == 0 && !*abort_flag)
           report_cluster(p.err, DEVERR_TIMEOUT_EPILOGUE, abort_flag, 2);
@@ -658,6 +698,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
   __syncthreads();
   ptx::cluster_sync_all();
   ptx::tc_fence_after();
+  // From here nobody issues any more, and a flag that was raised is raised in both CTAs.
+  if (*abort_flag) pair::drain(p, base, gbar, COUNT_AT, BOXES_AT, drain_bar, abort_flag);
   if (warp == 1) {
     __syncwarp();
     ptx::tmem_dealloc_pair(tmem_base, 512);
@@ -670,6 +712,31 @@ constexpr int THREADS = 192;   // producer, MMA issuer, four epilogue warps
 constexpr int TOK = 96;        // tokens of a tile at most: more leave too few stages
 constexpr int XTOK = 64;       // tokens of an exchange at most (SPLIT)
 constexpr int STEP = 2;        // k-blocks of a stage: one barrier round for both
+}  // namespace strm
+
+// What a CTA that gave up has under way, once its warps issue no more; all its threads.  `issued`
+// stages were filled.
+namespace strm {
+__device__ __noinline__ void drain(const Params& p, uint32_t bar_base, long long issued,
+                                   uint32_t drain_bar, volatile int* abort_flag) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, S = p.stages;
+  if (warp == 0 && lane == 0) {
+    for (long long f = max(0ll, issued - S); f < issued; ++f)
+      if (!ptx::mbar_wait(bar_base + 8u * (int)(f % S), (uint32_t)((f / S) & 1), nullptr, DRAIN_NS)) {
+        report(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag);
+        break;
+      }
+  }
+  __syncwarp();
+  if (warp == 1) {
+    if (ptx::elect_one()) ptx::umma_commit(drain_bar);
+    __syncwarp();
+    if (lane == 0 && !ptx::mbar_wait(drain_bar, 0, nullptr, DRAIN_NS))
+      report(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag);
+    __syncwarp();
+  }
+  __syncthreads();
+}
 }  // namespace strm
 
 // SPLIT: a cluster of csize CTAs cuts K.  The sums of a token go to the rank that finishes it,
@@ -708,6 +775,8 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
   const uint32_t rempty_bar = bar_base + 8u * (2 * MAX_STAGES + 6);  // every rank has read its
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gbar + 8 * (2 * MAX_STAGES + 7));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gbar + 8 * (2 * MAX_STAGES + 7) + 4);
+  constexpr int COUNT_AT = 8 * (2 * MAX_STAGES + 8);  // stages the producer filled
+  static_assert(COUNT_AT + 8 <= BAR_BYTES, "barriers and count");
   Table tb;
   tb.row0 = reinterpret_cast<int*>(gbar + BAR_BYTES);
   tb.cnt = tb.row0 + p.E;
@@ -805,13 +874,7 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
         if (++stage == S) { stage = 0; phase ^= 1u; }
       }
     }
-    if (lane == 0)
-      for (long long f = (issued > S ? issued - S : 0); f < issued; ++f) {
-        if (!ptx::mbar_wait(full_bar((int)(f % S)), (uint32_t)((f / S) & 1), nullptr, p.wait_ns)) {
-          report_cluster(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag, C);
-          break;
-        }
-      }
+    if (lane == 0) *reinterpret_cast<volatile long long*>(gbar + COUNT_AT) = issued;
     __syncwarp();
     if (SPLIT) ptx::cluster_arrive();
   } else if (warp == 1) {
@@ -819,7 +882,7 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
     int stage = 0;
     uint32_t phase = 0;
     int it = 0;
-    bool ok = true, issued_any = false;
+    bool ok = true;
     for (int tile = cid; ok && tile < T; tile += nclusters) {
       const Tile t = tile_of(p, tb, tile, p.band);
       const int ncol = (t.n + 15) / 16 * 16;
@@ -866,16 +929,9 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
             if (kb + nk >= s1) ptx::umma_commit(tfull_bar(a));
           }
           __syncwarp();
-          issued_any = true;
           if (++stage == S) { stage = 0; phase ^= 1u; }
         }
       }
-    }
-    if (!ok && issued_any) {
-      if (ptx::elect_one()) ptx::umma_commit(drain_bar);
-      __syncwarp();
-      if (lane == 0 && !ptx::mbar_wait(drain_bar, 0, nullptr, p.wait_ns))
-        report_cluster(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag, C);
     }
     __syncwarp();
     if (SPLIT) ptx::cluster_arrive();
@@ -887,7 +943,7 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
     const int slot = XT / C;    // tokens of a rank's slice at most
     const uint32_t tmem_q = tmem_base + ((uint32_t)(q * 32) << 16);
     const uint32_t send_q = send + (uint32_t)(q * XT) * 128u;  // this warp's part
-    int it = 0, xc = 0;         // accumulators read, exchanges made
+    int it = 0, xc = 0;         // accumulators read, exchanges that came in
     bool ok = true, arrived = false;
     for (int tile = cid; ok && tile < T; tile += nclusters) {
       const Tile t = tile_of(p, tb, tile, p.band);
@@ -903,7 +959,6 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
       // One exchange: tokens x0 .. x0 + xn of the tile, whose sums this warp has laid out.
       auto exchange = [&](int x0, int xn) {
         const uint32_t phase = (uint32_t)(xc & 1);
-        ++xc;
         const int per = (xn + C - 1) / C;          // rank r finishes tokens r * per ..
         const int mine = max(0, min(per, xn - rank * per));
         const int row0 = t.t0 + x0 + rank * per;
@@ -924,6 +979,7 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
         ok = ptx::mbar_wait_acquire_cluster(rfull_bar, phase, abort_flag, p.wait_ns);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) return;
+        ++xc;
         const bool last = last_tile && x0 + xn >= t.n;
         if (last) {  // this warp has made its last access to another CTA
           ptx::cluster_arrive();
@@ -983,7 +1039,8 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
       const int seg = SEG ? p.seg_kb : p.num_k_blocks;
       for (int s0 = kb0; ok && s0 < kb1; s0 += seg, ++it) {
         const int a = it & 1;
-        ok = ptx::mbar_wait(tfull_bar(a), (uint32_t)((it >> 1) & 1), abort_flag, p.wait_ns);
+        ok = ptx::mbar_wait(p.hold ? drain_bar : tfull_bar(a),
+                            p.hold ? 0u : (uint32_t)((it >> 1) & 1), abort_flag, p.wait_ns);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         ptx::tc_fence_after();
@@ -1007,14 +1064,22 @@ __global__ void __launch_bounds__(strm::THREADS, 1)
         report_cluster(p.err, DEVERR_TIMEOUT_EPILOGUE, abort_flag, C);
     }
     if (SPLIT && !arrived) {
+      // Given up: until the exchange that was next has come in whole, or for as long as a copy
+      // could conceivably take.  A warp that has sent its sums waits here or in the exchange for
+      // the other ranks', so no rank leaves while a copy from it or to it is under way.
+      if (!ok) ptx::mbar_wait_acquire_cluster(rfull_bar, (uint32_t)(xc & 1), nullptr, DRAIN_NS);
       __syncwarp();
       ptx::cluster_arrive();
     }
   }
 
   ptx::tc_fence_before();
-  __syncthreads();
+  const bool gave_up = __syncthreads_or(*abort_flag);
   ptx::tc_fence_after();
+  // Nobody here issues any more.  A flag that another rank raises later finds this CTA's work
+  // done: its epilogue has seen every accumulator.
+  if (gave_up)
+    strm::drain(p, bar_base, *reinterpret_cast<volatile long long*>(gbar + COUNT_AT), drain_bar, abort_flag);
   if (warp == 1) {
     __syncwarp();
     ptx::tmem_dealloc(tmem_base, tmem_cols);
@@ -1188,6 +1253,7 @@ qgemm_status launch_linear_tcgen05(qgemm_stream_s* s, const LinArgs& a) {
   p.num_k_blocks = (int)(((long long)a.K * es + BK - 1) / BK);
   p.err = s->dev->d_err;
   p.bad = s->index_word;
+  p.hold = s->dev->hold_split;
   p.wait_ns = s->dev->wait_ns;
   p.rows = WROWS;
   const int table = ((3 * a.E + 1) * 4 + 15) / 16 * 16;

@@ -109,18 +109,20 @@ QGEMM_API qgemm_status qgemm_device_close(qgemm_device_t dev);
 /* sm_count, compute capability, L2 bytes, and whether tcgen05 kernels run. */
 QGEMM_API qgemm_status qgemm_device_info(qgemm_device_t dev, int* sm_count, int* cc_major,
                                int* cc_minor, size_t* l2_bytes, int* has_tcgen05);
-/* Limit, in nanoseconds of the GPU's global timer, of every bounded device-side wait
- * in the tensor-core GEMM kernels (W8A8, bf16, fp32 entry points) launched on this
- * device from now on; default 2 s, accepted range 1 us .. 60 s.  A wait that runs out
- * ends its kernel early and qgemm_stream_sync() then reports QGEMM_ERR_TIMEOUT.  No
- * counterpart in the reference, whose launches never wait on the device. */
+/* Limit, in nanoseconds of the GPU's global timer, of every bounded device-side wait in the
+ * tensor-core GEMM kernels (W8A8, bf16, fp32 entry points) and linear layers launched on this
+ * device from now on; default 2 s, accepted range 1 us .. 60 s.  A wait that runs out ends its
+ * kernel early and qgemm_stream_sync() then reports QGEMM_ERR_TIMEOUT.  (A linear layer that
+ * gives up still waits for its own copies and tensor-core work, up to 2 s.)  No counterpart in
+ * the reference, whose launches never wait on the device. */
 QGEMM_API qgemm_status qgemm_device_set_wait_limit(qgemm_device_t dev, uint64_t limit_ns);
 QGEMM_API qgemm_status qgemm_device_get_wait_limit(qgemm_device_t dev, uint64_t* limit_ns);
 /* Test hook for the timeout path (no counterpart in the reference): with enable != 0,
  * the final K part of every tile the W8A8 GEMM's last-wave split cuts waits for one
  * count-in more than the other parts make, so its bounded wait runs out after the
- * device's wait limit; the call then ends in QGEMM_ERR_TIMEOUT at qgemm_stream_sync()
- * (its output is undefined) and the stream stays usable.  Leave it off otherwise. */
+ * device's wait limit, and so do the epilogues of the linear layers on the tensor cores; the
+ * call then ends in QGEMM_ERR_TIMEOUT at qgemm_stream_sync() (its output is undefined) and the
+ * stream stays usable.  Leave it off otherwise. */
 QGEMM_API qgemm_status qgemm_debug_hold_split(qgemm_device_t dev, int enable);
 
 /* ---- streams ---------------------------------------------------------------

@@ -85,6 +85,11 @@ qgemm_status linear_entry(qgemm_stream_t s, int kind, uint64_t x, int ldx, uint6
   if (K > 0 && (overlap(o, range_of(x, M, (unsigned long long)ldx * es, (unsigned long long)K * es)) ||
                 overlap(o, range_of(w, nw * E, (unsigned long long)K * es, (unsigned long long)K * es))))
     return fail(QGEMM_ERR_INVALID_ARG, "out overlaps an operand");
+  const auto run = [](uint64_t p, unsigned long long bytes) { return Range{p, p + bytes}; };
+  if ((kind == KIND_I8 && (overlap(o, run(sx, 4ull * M)) || overlap(o, run(sw, 4ull * nw * E)))) ||
+      (bias && overlap(o, run(bias, 4ull * nw * E))) ||
+      (experts && overlap(o, run(offsets, 4ull * (E + 1)))))
+    return fail(QGEMM_ERR_INVALID_ARG, "out overlaps the scales, the bias or the offsets");
   if (residual && !(residual == out && ldr == ldc) &&
       overlap(o, range_of(residual, M, (unsigned long long)ldr * os, (unsigned long long)N * os)))
     return fail(QGEMM_ERR_INVALID_ARG, "out overlaps the residual without being it");

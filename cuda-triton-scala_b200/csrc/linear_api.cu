@@ -26,6 +26,29 @@ Range range_of(uint64_t p, long long rows, unsigned long long pitch, unsigned lo
 
 bool overlap(const Range& a, const Range& b) { return a.lo < b.hi && b.lo < a.hi; }
 
+// `rows` rows of `width` bytes, `pitch` bytes apart.
+struct Rows {
+  uint64_t p;
+  long long rows;
+  unsigned long long pitch, width;
+};
+
+// Whether two buffers share a byte.  Exact for rows of one pitch (columns of one wider buffer) and
+// where one is a single run; else the ranges from first to last byte are compared.
+bool overlap(const Rows& a, const Rows& b) {
+  if (!overlap(range_of(a.p, a.rows, a.pitch, a.width), range_of(b.p, b.rows, b.pitch, b.width)))
+    return false;
+  if (a.rows > 1 && b.rows > 1 && a.pitch != b.pitch) return true;
+  const unsigned long long pitch = a.rows > 1 ? a.pitch : b.pitch;
+  if (a.rows == 1 && b.rows == 1) return true;
+  const Rows& first = a.p <= b.p ? a : b;
+  const Rows& second = a.p <= b.p ? b : a;
+  const unsigned long long d = (second.p - first.p) % pitch;
+  // a single run that begins first and reaches the other holds its first byte
+  if (first.rows == 1) return true;
+  return d < first.width || d + second.width > pitch;
+}
+
 qgemm_status need(uint64_t p, uint64_t align, const char* name) {
   if (p == 0) return fail(QGEMM_ERR_INVALID_ARG, "%s is null", name);
   if (!aligned(p, align))
@@ -81,17 +104,20 @@ qgemm_status linear_entry(qgemm_stream_t s, int kind, uint64_t x, int ldx, uint6
   if (bias) QG_TRY(need(bias, 4, "bias"));
   if (residual) QG_TRY(need(residual, os, "residual"));
   if (experts) QG_TRY(need(offsets, 4, "offsets"));
-  const Range o = range_of(out, M, (unsigned long long)ldc * os, (unsigned long long)N * os);
-  if (K > 0 && (overlap(o, range_of(x, M, (unsigned long long)ldx * es, (unsigned long long)K * es)) ||
-                overlap(o, range_of(w, nw * E, (unsigned long long)K * es, (unsigned long long)K * es))))
+  const auto rows = [](uint64_t p, long long n, unsigned long long pitch, unsigned long long width) {
+    return Rows{p, n, pitch, width};
+  };
+  const auto run = [](uint64_t p, unsigned long long bytes) { return Rows{p, 1, bytes, bytes}; };
+  const Rows o = rows(out, M, (unsigned long long)ldc * os, (unsigned long long)N * os);
+  if (K > 0 && (overlap(o, rows(x, M, (unsigned long long)ldx * es, (unsigned long long)K * es)) ||
+                overlap(o, run(w, (unsigned long long)(nw * E) * K * es))))
     return fail(QGEMM_ERR_INVALID_ARG, "out overlaps an operand");
-  const auto run = [](uint64_t p, unsigned long long bytes) { return Range{p, p + bytes}; };
   if ((kind == KIND_I8 && (overlap(o, run(sx, 4ull * M)) || overlap(o, run(sw, 4ull * nw * E)))) ||
       (bias && overlap(o, run(bias, 4ull * nw * E))) ||
       (experts && overlap(o, run(offsets, 4ull * (E + 1)))))
     return fail(QGEMM_ERR_INVALID_ARG, "out overlaps the scales, the bias or the offsets");
   if (residual && !(residual == out && ldr == ldc) &&
-      overlap(o, range_of(residual, M, (unsigned long long)ldr * os, (unsigned long long)N * os)))
+      overlap(o, rows(residual, M, (unsigned long long)ldr * os, (unsigned long long)N * os)))
     return fail(QGEMM_ERR_INVALID_ARG, "out overlaps the residual without being it");
   QG_TRY(enter(s));
   LinArgs a;

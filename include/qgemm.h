@@ -441,7 +441,7 @@ QGEMM_API qgemm_status qgemm_gemv_f32(qgemm_stream_t s, uint64_t A, uint64_t x, 
  * QGEMM_ALGO_TCGEN05 refuses what the tensor cores cannot take (QGEMM_ERR_UNSUPPORTED).
  * M == 0 or N == 0 does nothing.  M, N, K <= 2^30.  int8: K <= 131071 (the int32 sums cannot overflow).
  * `out` may not overlap x, w, the scales, the bias, the offsets or (unless it is the same
- * buffer) the residual. */
+ * buffer) the residual; columns of one wider buffer, rows of one pitch, do not overlap. */
 QGEMM_API qgemm_status qgemm_linear_bf16_nk(qgemm_stream_t s, uint64_t x, int ldx, uint64_t w,
                                             uint64_t bias, uint64_t residual, int ldr,
                                             uint64_t out, int out_dtype, int ldc, int M, int N,

@@ -220,12 +220,12 @@ def addr(x) -> int:
     Ptr.address), an object with ``.address`` or a torch tensor (data_ptr)."""
     if x is None:
         return 0
-    try:
-        return x.data_ptr()
-    except AttributeError:
-        pass
     if isinstance(x, int):
         return x
-    if hasattr(x, "address"):
-        return int(x.address)
+    data_ptr = getattr(x, "data_ptr", None)
+    if data_ptr is not None:
+        return data_ptr()
+    address = getattr(x, "address", None)
+    if address is not None:
+        return int(address)
     raise TypeError(f"cannot take a device address of {type(x).__name__}")

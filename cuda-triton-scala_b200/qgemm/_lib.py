@@ -215,17 +215,25 @@ def try_call(name: str, *args) -> int:
     return int(getattr(lib(), name)(*args))
 
 
+_tensor_types: set = set()  # types met whose instances have data_ptr()
+
+
 def addr(x) -> int:
     """Device address of a Ptr-like argument: an int address (the reference's
     Ptr.address), an object with ``.address`` or a torch tensor (data_ptr)."""
     if x is None:
         return 0
+    t = type(x)
+    if t in _tensor_types:
+        return x.data_ptr()
     if isinstance(x, int):
         return x
-    data_ptr = getattr(x, "data_ptr", None)
-    if data_ptr is not None:
-        return data_ptr()
+    if hasattr(t, "data_ptr"):
+        _tensor_types.add(t)
+        return x.data_ptr()
     address = getattr(x, "address", None)
     if address is not None:
         return int(address)
+    if hasattr(x, "data_ptr"):  # a proxy
+        return x.data_ptr()
     raise TypeError(f"cannot take a device address of {type(x).__name__}")

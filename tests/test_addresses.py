@@ -37,3 +37,16 @@ def test_an_error_of_data_ptr_is_not_hidden():
 
     with pytest.raises(AttributeError, match="no storage"):
         L.addr(Tensor())
+
+
+def test_a_proxy_of_a_tensor():
+    class Proxy:
+        def __init__(self, inner):
+            self._inner = inner
+
+        def __getattr__(self, name):
+            return getattr(self._inner, name)
+
+    torch = pytest.importorskip("torch")
+    t = torch.empty(4)
+    assert L.addr(Proxy(t)) == t.data_ptr()

@@ -130,3 +130,28 @@ def test_many_stream_handles_keep_their_errors_apart(gpu):
     finally:
         for st in held:
             st.destroy()
+
+
+def test_more_handles_than_words(gpu):
+    """Past 4095 handles at a time the last word is shared: errors still reach the handle that
+    called, if it is the next of them to be synchronised."""
+    dev, _, _ = gpu
+    own = dev.stream()
+    raw = torch.cuda.Stream().cuda_stream
+    held = [dev.wrap_stream(raw) for _ in range(4200)]
+    try:
+        for i in (10, 4199):
+            keep = bad_combine(qgemm.QuantizedGemmOps(held[i]))
+            torch.cuda.synchronize()
+            own.sync()
+            with pytest.raises(qgemm.QGemmError):
+                held[i].sync()
+            held[i].sync()
+            del keep
+    finally:
+        for st in held:
+            st.destroy()
+    own.destroy()
+    st = dev.stream()
+    st.sync()
+    st.destroy()

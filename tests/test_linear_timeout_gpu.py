@@ -49,3 +49,36 @@ def test_a_wait_that_runs_out_ends_the_call_and_the_stream_goes_on(gpu, name):
         st.sync()
         c.check()
     st.destroy()
+
+
+@pytest.mark.parametrize("name", sorted(CASES))
+@pytest.mark.parametrize("limit", [1000, 4000])
+def test_limits_shorter_than_a_copy(gpu, name, limit):
+    """A limit of a few microseconds runs out in any wait, at any point, in one CTA of a pair or
+    cluster before the other: the call ends all the same, and is right or reported."""
+    dev, _, _ = gpu
+    kind, M, N, K, more = CASES[name]
+    c = Case(kind, M, N, K, **more)
+    st = dev.stream()
+    ops = qgemm.QuantizedGemmOps(st)
+    old = dev.wait_limit_ns
+    for _ in range(3):
+        c.out.fill_(-77.25)
+        torch.cuda.synchronize()
+        dev.wait_limit_ns = limit
+        try:
+            c.call(ops, qgemm.ALGO_TCGEN05)
+            try:
+                st.sync()
+                c.check()
+            except qgemm.QGemmError as e:
+                assert e.status == qgemm._lib.ERR_TIMEOUT
+        finally:
+            dev.wait_limit_ns = old
+        st.sync()
+    c.out.fill_(-77.25)
+    torch.cuda.synchronize()
+    c.call(ops, qgemm.ALGO_TCGEN05)
+    st.sync()
+    c.check()
+    st.destroy()

@@ -14,15 +14,18 @@
 //
 //   linear_pair_kernel    many rows: CTA pairs (tcgen05 cta_group::2), tiles of 256 weight
 //       rows x up to 256 tokens, persistent, two accumulators so that the epilogue of a tile
-//       overlaps the next tile's MMAs.  Bound by the tensor pipe and, under sustained load, by
-//       the power cap: int8 gated 8192 x 28672 x 4096 0.68 ms (2.83 POPS), bf16 4096 x 4096 x
-//       11008 with bias, gelu and residual 265 to 280 us (1.32 to 1.39 PFLOP/s).
+//       overlaps the next tile's MMAs.  Bound by the tensor pipe and, after seconds of load, by
+//       the power cap: int8 gated 8192 x 28672 x 4096 0.57 ms (3.38 POPS; 0.68 under the cap),
+//       bf16 4096 x 4096 x 11008 with bias, gelu and residual 261 to 264 us (1.41 PFLOP/s; 322).
+//       Ungated, the epilogue spills (about 450 bytes a thread at the 168 registers that ten
+//       warps leave), which shows where few k-blocks hide it: 4976 x 1728 x 328 19 us, with GELU
+//       36.
 //   linear_stream_kernel  few rows: one CTA per tile of up to 128 weight rows x up to 96
 //       tokens, two k-blocks a stage, persistent; a cluster of 1, 2, 4 or 8 CTAs cuts K and
 //       joins its partial sums through distributed shared memory in rank order (so no scratch,
 //       no atomics, the same bits every time).  Bound by reading the weights once: 940 MB of
 //       experts' weights in 143 us (6.6 TB/s); small layers by 3.4 us of launch, first copy and
-//       exchange (1 x 4096 x 4096 bf16: 8.9 us).
+//       exchange (1 x 4096 x 4096 bf16 with bias and residual: 8.7 us).
 //
 // Experts: offsets[E + 1] are read on the device; every CTA lists the experts' tiles in
 // shared memory (prefix sums) and walks the same persistent schedule, so the host never

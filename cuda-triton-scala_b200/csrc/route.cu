@@ -272,7 +272,8 @@ __global__ void __launch_bounds__(1024, 1)
 // ---- dispatch -----------------------------------------------------------------------
 
 // out[rows[t, j]] = x[t]: each thread holds one piece (16 bytes, or one element) of a token
-// row and stores it to the token's k places; x is read once.
+// row and stores it to the token's k places; x is read once.  Bound by HBM where rows are whole
+// pieces (8192 tokens x 2 bf16: K = 4096 32 us, floor 31; K = 4095, an element a thread, 137).
 template <typename V>
 __global__ void __launch_bounds__(256) dispatch_copy_kernel(const V* __restrict__ x,
                                                             const int* __restrict__ rows,
@@ -301,8 +302,9 @@ __device__ __forceinline__ int8_t quant(float v, float mul) {
 }
 
 // A token per CTA, quantised once and stored to its k places.  NV > 0: the row is held in
-// registers (NV pieces of 4 elements a thread; K % 4 == 0 and aligned rows); NV = 0: any row,
-// read twice.  maxAbs in the "if (v > m) m = v" form: a NaN never replaces a number.
+// registers (NV pieces of 4 elements a thread: K % 4 == 0, aligned rows, K <= 8192); NV = 0: any
+// row, read once for the maximum and again, and quantised, for each place (8192 tokens x 2 bf16: K =
+// 4096 28 us, 4095 46; 8192 58, 8196 77).  maxAbs in the "if (v > m) m = v" form: a NaN never replaces a number.
 template <typename T, int NV>
 __global__ void __launch_bounds__(256) dispatch_quant_kernel(const T* __restrict__ x,
                                                              const int* __restrict__ rows,
@@ -436,7 +438,8 @@ __device__ __forceinline__ void store8(T* __restrict__ p, int left, const float 
 
 // out[t] = sum_j w[t, j] y[rows[t, j]] (+ residual[t]): a thread per 8 columns of a token,
 // fp32 sums with j ascending.  Bound by HBM: U rows' loads are in flight a thread, as loaded
-// (8 rows of bf16: 172 us at 8192 tokens of 8 rows x 4096 with 4 in flight and widened at once).
+// (8 rows of bf16: 172 us at 8192 tokens of 8 rows x 4096 with 4 in flight and widened at once, 114
+// to 119 this way).  Widths that are not a multiple of 8 go element by element (4095: 201 us).
 template <typename TI, typename TO, bool VEC, int U>
 __global__ void __launch_bounds__(128) combine_kernel(const TI* __restrict__ y,
                                                       const int* __restrict__ rows,

@@ -499,7 +499,7 @@ QGEMM_API qgemm_status qgemm_w8a8_expert_linear(qgemm_stream_t s, uint64_t A, in
  *
  * rows[t,j] < 0 names no row (nothing is written, nothing added); a row >= R is skipped and
  * the next qgemm_stream_sync of this handle reports QGEMM_ERR_INVALID_ARG.  Two pairs that name one row
- * leave either's values there.  Outputs may not overlap inputs, but for the residual. */
+ * leave a mixture of theirs there.  Outputs may not overlap inputs, but for the residual. */
 QGEMM_API qgemm_status qgemm_route_topk(qgemm_stream_t s, uint64_t logits, int in_dtype,
                                         uint64_t weights, uint64_t experts, uint64_t offsets,
                                         uint64_t rows, int T, int E, int k, int renormalize);

@@ -196,7 +196,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
         if (rank == 0) {  // the copies in flight land before the CTA may exit
           for (long long f = (issued > STAGES ? issued - STAGES : 0); f < issued; ++f) {
             if (!ptx::mbar_wait(full_bar((int)(f % STAGES)), (uint32_t)((f / STAGES) & 1),
-                                nullptr, p.wait_ns)) {
+                                nullptr)) {
               report(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag, rank);
               break;
             }
@@ -247,9 +247,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
             if (ok) ptx::umma_commit_pair(tfull_bar(a), 0x3);
           }
         }
-        if (!ok && issued_any) {
+        if (issued_any) {  // before TMEM is released: an epilogue that gave up has not waited
           ptx::umma_commit_pair(drain_bar, 0x1);
-          if (!ptx::mbar_wait(drain_bar, 0, nullptr, p.wait_ns))
+          if (!ptx::mbar_wait(drain_bar, 0, nullptr))
             report(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag, rank);
         }
       }

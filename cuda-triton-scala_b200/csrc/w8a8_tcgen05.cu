@@ -561,7 +561,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       for (long long f = (issued > STAGES ? issued - STAGES : 0); f < issued; ++f) {
         const int s = (int)(f % STAGES);
         const uint32_t par = (uint32_t)((f / STAGES) & 1);
-        if (!ptx::mbar_wait(full_bar(s), par, nullptr, p.wait_ns)) {
+        if (!ptx::mbar_wait(full_bar(s), par, nullptr)) {
           report(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag);
           break;
         }
@@ -623,10 +623,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
         if (ok) ptx::umma_commit(tfull_bar(a));
       }
-      if (!ok && issued_any) {
-        // Wait for the MMAs already issued before TMEM is released.
+      if (issued_any) {
+        // Wait for every MMA issued before TMEM is released: an epilogue that gave up has not.
         ptx::umma_commit(drain_bar);
-        if (!ptx::mbar_wait(drain_bar, 0, nullptr, p.wait_ns)) report(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag);
+        if (!ptx::mbar_wait(drain_bar, 0, nullptr)) report(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag);
       }
     }
   } else {
@@ -795,7 +795,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
       // Drain: the even CTA's full barriers count both CTAs' copies.
       if (rank == 0) {
         for (long long f = (issued > STAGES ? issued - STAGES : 0); f < issued; ++f) {
-          if (!ptx::mbar_wait(full_bar((int)(f % STAGES)), (uint32_t)((f / STAGES) & 1), nullptr, p.wait_ns)) {
+          if (!ptx::mbar_wait(full_bar((int)(f % STAGES)), (uint32_t)((f / STAGES) & 1), nullptr)) {
             report_pair(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag, rank);
             break;
           }
@@ -865,9 +865,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
         }
         if (ok) ptx::umma_commit_pair(tfull_bar(a), 0x3);
       }
-      if (!ok && issued_any) {
+      if (issued_any) {
+        // Wait for every MMA issued before TMEM is released: an epilogue that gave up has not.
         ptx::umma_commit_pair(drain_bar, 0x1);
-        if (!ptx::mbar_wait(drain_bar, 0, nullptr, p.wait_ns)) report_pair(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag, rank);
+        if (!ptx::mbar_wait(drain_bar, 0, nullptr)) report_pair(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag, rank);
       }
     }
   } else {

@@ -38,3 +38,32 @@ def test_bf16_outputs_of_very_long_sums(gpu, M, experts):
     got = out[rows].double()
     inside = (got >= lo) & (got <= hi)
     assert inside.all(), f"{int((~inside).sum())} of {inside.numel()} outside"
+
+
+@pytest.mark.parametrize("M,gated", [(2, False), (2, True), (40, True), (300, False), (300, True)])
+@pytest.mark.parametrize("experts", [False, True])
+def test_bf16_outputs_in_pieces_with_every_epilogue(gpu, M, gated, experts):
+    """K = 66048, past where bf16 outputs are summed in pieces; small integers, whose sums are exact
+    (9 K < 2^24), so the epilogue's tolerance alone is left."""
+    from test_linear_gpu import Case, run
+    off = [0, M // 3, M // 3, M] if experts else None
+    run(gpu, Case("bf16", M, 203, 66048, act="gelu", gated=gated, bias=True, residual=not experts,
+                  offsets=off), qgemm.ALGO_TCGEN05)
+
+
+@pytest.mark.parametrize("K", [131056, 131071])
+def test_int8_sums_at_their_largest(gpu, K):
+    """All of x and w at -128: the int32 sum is K 2^14, just below 2^31 (131056 on the tensor cores,
+    131071 on CUDA cores); the scales are powers of two, so one rounding to fp32 is left."""
+    _, st, ops = gpu
+    M, N = 3, 40
+    x = torch.full((M, K), -128, dtype=torch.int8, device="cuda")
+    w = torch.full((N, K), -128, dtype=torch.int8, device="cuda")
+    sx = torch.full((M,), 2.0 ** -10, device="cuda")
+    sw = torch.full((N,), 2.0 ** -7, device="cuda")
+    out = torch.empty(M, N, device="cuda")
+    torch.cuda.synchronize()
+    ops.w8a8Linear(x, w, sx, sw, out, M, N, K, out_dtype=qgemm.F32)
+    st.sync()
+    want = torch.tensor(float(K * 2 ** 14), dtype=torch.float64).float().item() * 2.0 ** -17
+    assert (out == want).all()

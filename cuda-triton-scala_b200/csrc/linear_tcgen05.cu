@@ -45,6 +45,7 @@
 
 #include "linear_epilogue.cuh"
 #include "linear_tiles.cuh"
+#include "pair_copies.cuh"
 #include "ptx.cuh"
 
 namespace qg {
@@ -117,9 +118,6 @@ __device__ __forceinline__ void fill_table(const Params& p, const Table& tb) {
   }
   __syncthreads();
 }
-
-// Limit of the waits for this CTA's own copies and MMAs after it has given up.
-constexpr unsigned long long DRAIN_NS = ptx::kWaitLimitNs;
 
 __device__ __forceinline__ void report(int* err, int code, volatile int* abort_flag) {
   *abort_flag = 1;
@@ -419,33 +417,12 @@ constexpr int SEG_TOK = 128;              // tokens of a tile at most with SEG
 // abort flag; all threads of both.  (Out of line, as the stream kernel's: inline it lay between
 // the hot code and the exit, and cost small calls 0.3 us of instruction fetch.)
 namespace pair {
-__device__ __noinline__ void drain(const Params& p, uint32_t base, const uint8_t* gbar, int count_at,
-                                   int boxes_at, uint32_t drain_bar, volatile int* abort_flag) {
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, S = p.stages;
+__device__ __noinline__ void drain(const Params& p, uint32_t bar_base, uint32_t copies,
+                                   uint32_t drain_bar, volatile int* abort_flag) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t rank = ptx::cluster_ctarank();
-  auto full_bar = [&](int s) { return base + S * STAGE_BYTES + 8u * s; };
-  if (warp == 0 && rank == 0 && lane == 0) {
-    // The even CTA's full barriers count both CTAs' copies.  Where one producer got further than
-    // the other, the missing half of a stage is taken off its count (the even CTA armed it for
-    // both), or the half that is on its way armed alone.
-    const uint32_t there = ptx::map_to_rank(base + S * STAGE_BYTES, 1);
-    const long long mine = *reinterpret_cast<const volatile long long*>(gbar + count_at);
-    const long long theirs = ptx::ld_cluster_s64(there + count_at);
-    const long long first = min(mine, theirs), end = max(mine, theirs);
-    for (long long f = first; f < end; ++f) {
-      const int at = (int)(f % S);
-      const uint32_t boxes = mine > theirs ? (uint32_t)gbar[boxes_at + at]
-                                           : ptx::ld_cluster_u8(there + boxes_at + at);
-      const uint32_t half = W_BYTES + boxes * BOX * BK;
-      if (mine > theirs) ptx::mbar_complete_tx(full_bar(at), half);
-      else ptx::mbar_arrive_expect_tx(full_bar(at), half);
-    }
-    for (long long f = max(0ll, end - S); f < end; ++f)
-      if (!ptx::mbar_wait(full_bar((int)(f % S)), (uint32_t)((f / S) & 1), nullptr, DRAIN_NS)) {
-        report(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag);
-        break;
-      }
-  }
+  if (warp == 0 && rank == 0 && lane == 0 && !settle_pair_copies(bar_base, p.stages, copies))
+    report(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag);
   __syncwarp();
   if (warp == 1) {  // everything that the even CTA's issuer has committed, in both CTAs
     if (rank == 0 && ptx::elect_one()) ptx::umma_commit_pair(drain_bar, 0x3);
@@ -480,10 +457,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
   const uint32_t drain_bar = bar_base + 8u * (2 * MAX_STAGES + 4);
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gbar + 8 * (2 * MAX_STAGES + 5));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gbar + 8 * (2 * MAX_STAGES + 5) + 4);
-  // stages this CTA's producer filled, and the token boxes of the last one in each place: what
-  // the drain needs of both CTAs
-  constexpr int COUNT_AT = 8 * (2 * MAX_STAGES + 6), BOXES_AT = COUNT_AT + 8;
-  static_assert(BOXES_AT + MAX_STAGES <= BAR_BYTES, "barriers and counts");
+  constexpr int COPIES_AT = 8 * (2 * MAX_STAGES + 6);
+  static_assert(COPIES_AT + (int)sizeof(PairCopies) <= BAR_BYTES, "barriers and counts");
+  static_assert((SMEM_MAX - BAR_BYTES) / pair::STAGE_BYTES <= 8, "stages that PairCopies holds");
+  PairCopies* copies = reinterpret_cast<PairCopies*>(gbar + COPIES_AT);
   Table tb;
   tb.row0 = reinterpret_cast<int*>(gbar + BAR_BYTES);
   tb.cnt = tb.row0 + p.E;
@@ -544,7 +521,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
           break;
         }
         if (ptx::elect_one()) {
-          gbar[BOXES_AT + stage] = (uint8_t)boxes;
+          copies->half[stage] = tx / 2;
           const uint32_t sw = base + stage * pair::STAGE_BYTES, sx = sw + W_BYTES;
           const uint32_t fb = ptx::map_to_rank(full_bar(stage), 0);
           if (rank == 0) ptx::mbar_arrive_expect_tx(full_bar(stage), tx);
@@ -576,7 +553,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
         if (++stage == S) { stage = 0; phase ^= 1u; }
       }
     }
-    if (lane == 0) *reinterpret_cast<volatile long long*>(gbar + COUNT_AT) = issued;
+    if (lane == 0) copies->stages = issued;
   } else if (warp == 1) {
     // ---------------- MMA issuer (even CTA) ----------------
     if (rank == 0) {
@@ -702,7 +679,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::THREADS, 1)
   ptx::cluster_sync_all();
   ptx::tc_fence_after();
   // From here nobody issues any more, and a flag that was raised is raised in both CTAs.
-  if (*abort_flag) pair::drain(p, base, gbar, COUNT_AT, BOXES_AT, drain_bar, abort_flag);
+  if (*abort_flag) pair::drain(p, bar_base, bar_base + COPIES_AT, drain_bar, abort_flag);
   if (warp == 1) {
     __syncwarp();
     ptx::tmem_dealloc_pair(tmem_base, 512);

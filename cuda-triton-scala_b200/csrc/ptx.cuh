@@ -233,10 +233,10 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t smem_addr, uint32_t ran
   return r;
 }
 
-// 1 and 8 bytes from shared memory anywhere in the cluster (addresses from map_to_rank).
-__device__ __forceinline__ uint32_t ld_cluster_u8(uint32_t cluster_addr) {
+// 4 and 8 bytes from shared memory anywhere in the cluster (addresses from map_to_rank).
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t cluster_addr) {
   uint32_t v;
-  asm volatile("ld.shared::cluster.u8 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory");
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory");
   return v;
 }
 __device__ __forceinline__ long long ld_cluster_s64(uint32_t cluster_addr) {

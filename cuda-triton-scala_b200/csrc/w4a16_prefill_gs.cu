@@ -40,6 +40,7 @@
 #include <mutex>
 
 #include "internal.h"
+#include "pair_copies.cuh"
 #include "ptx.cuh"
 
 namespace qg {
@@ -131,6 +132,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
   const uint32_t drain_bar = bar_base + 8u * (2 * STAGES + 4);
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gbar + 8 * (2 * STAGES + 5));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gbar + 8 * (2 * STAGES + 5) + 4);
+  constexpr int COPIES_AT = 8 * (2 * STAGES + 6);
+  static_assert(COPIES_AT + (int)sizeof(PairCopies) <= BAR_BYTES && STAGES <= 8, "barriers and counts");
+  PairCopies* copies = reinterpret_cast<PairCopies*>(gbar + COPIES_AT);
 
   const int warp = threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
@@ -186,6 +190,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
             }
             const uint32_t sa = base + stage * STAGE_BYTES;
             const uint32_t fb = ptx::map_to_rank(full_bar(stage), 0);
+            copies->half[stage] = STAGE_BYTES;
             if (rank == 0) ptx::mbar_arrive_expect_tx(full_bar(stage), 2 * STAGE_BYTES);
             ptx::tma_load_2d_pair(sa, &tmA, fb, kb * BK, mb * 256 + (int)rank * 128);
             ptx::tma_load_2d_pair(sa + A_BYTES, &tmB, fb, kb * BK, nb * 256 + (int)rank * 128);
@@ -193,15 +198,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
             if (++stage == STAGES) { stage = 0; phase ^= 1u; }
           }
         }
-        if (rank == 0) {  // the copies in flight land before the CTA may exit
-          for (long long f = (issued > STAGES ? issued - STAGES : 0); f < issued; ++f) {
-            if (!ptx::mbar_wait(full_bar((int)(f % STAGES)), (uint32_t)((f / STAGES) & 1),
-                                nullptr)) {
-              report(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag, rank);
-              break;
-            }
-          }
-        }
+        copies->stages = issued;
       }
     } else if (warp == 1) {
       // ---------------- MMA issuer (even CTA) ----------------
@@ -380,6 +377,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
   __syncthreads();
   ptx::cluster_sync_all();  // the pair's MMAs and remote arrivals are finished
   ptx::tc_fence_after();
+  // A pair that gave up (the flag is raised in both CTAs): neither leaves before its copies have
+  // landed.  Otherwise the MMAs have read every stage.  (By an epilogue warp, which has the
+  // registers.)
+  if (*abort_flag) {
+    if (rank == 0 && threadIdx.x == 32 * EPI_WARP0 &&
+        !settle_pair_copies(bar_base, STAGES, bar_base + COPIES_AT) && p.err)
+      atomicCAS(p.err, 0, DEVERR_TIMEOUT_DRAIN);
+    __syncthreads();
+    ptx::cluster_sync_all();
+  }
   if (warp == 1) {
     __syncwarp();
     ptx::tmem_dealloc_pair(tmem_base, TMEM_COLS);

@@ -36,6 +36,7 @@
 #include <mutex>
 
 #include "internal.h"
+#include "pair_copies.cuh"
 #include "ptx.cuh"
 
 namespace qg {
@@ -230,6 +231,15 @@ __device__ __forceinline__ void report_pair(int* err, int code, volatile int* ab
   report(err, code, abort_flag);
   const uint32_t peer = ptx::map_to_rank(ptx::smem_u32(const_cast<int*>(abort_flag)), rank ^ 1u);
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer), "r"(1) : "memory");
+}
+
+// All threads of a pair that gave up, once neither CTA issues any more.
+__device__ __noinline__ void drain_copies(int* err, uint32_t full0, int stages, uint32_t copies,
+                                          uint32_t rank) {
+  if (rank == 0 && threadIdx.x == 0 && !settle_pair_copies(full0, stages, copies) && err)
+    atomicCAS(err, 0, DEVERR_TIMEOUT_DRAIN);
+  __syncthreads();
+  ptx::cluster_sync_all();
 }
 
 // The int32 accumulators of 32 consecutive columns of one row (row < M, n0 < N), plus
@@ -717,6 +727,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
   uint8_t* gbar = gbase + STAGES * STAGE_BYTES + STG_BYTES;
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gbar + 8 * (2 * STAGES + 5));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(gbar + 8 * (2 * STAGES + 5) + 4);
+  constexpr int COPIES_AT = 8 * (2 * STAGES + 7);  // past the slot, the flag and last_flag
+  static_assert(COPIES_AT + (int)sizeof(PairCopies) <= BAR_BYTES && STAGES <= 8, "barriers and counts");
+  PairCopies* copies = reinterpret_cast<PairCopies*>(gbar + COPIES_AT);
 
   const int warp = threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
@@ -782,6 +795,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
           const uint32_t fb = ptx::map_to_rank(full_bar(stage), 0);
           int akb, bkb;
           seg_blocks(p, kb, akb, bkb);
+          copies->half[stage] = tx / 2;
           if (rank == 0) ptx::mbar_arrive_expect_tx(full_bar(stage), tx);
           ptx::tma_load_2d_pair(sa, &tmA, fb, akb * BK, mb * BM + (int)rank * 128);
           if (p.b_kn)
@@ -792,15 +806,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
           if (++stage == STAGES) { stage = 0; phase ^= 1u; }
         }
       }
-      // Drain: the even CTA's full barriers count both CTAs' copies.
-      if (rank == 0) {
-        for (long long f = (issued > STAGES ? issued - STAGES : 0); f < issued; ++f) {
-          if (!ptx::mbar_wait(full_bar((int)(f % STAGES)), (uint32_t)((f / STAGES) & 1), nullptr)) {
-            report_pair(p.err, DEVERR_TIMEOUT_DRAIN, abort_flag, rank);
-            break;
-          }
-        }
-      }
+      copies->stages = issued;
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer (even CTA) ----------------
@@ -984,6 +990,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
   __syncthreads();
   ptx::cluster_sync_all();  // the pair's MMAs and remote arrivals are finished
   ptx::tc_fence_after();
+  // A pair that gave up (the flag is raised in both CTAs): neither leaves before its copies have
+  // landed.  Otherwise the MMAs have read every stage.
+  if (*abort_flag) drain_copies(p.err, bar_base, STAGES, bar_base + COPIES_AT, rank);
   if (warp == 1) {
     __syncwarp();
     ptx::tmem_dealloc_pair(tmem_base, TMEM_COLS);
